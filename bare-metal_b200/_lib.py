@@ -42,6 +42,11 @@ SIGNATURES = {
     "bm_sp_pack_weights": (_i, [_p, _p, _i, _p, _i, _i, _p]),
     "bm_w8a8_sparse_i32_packed": (_i, [_p, _p, _p, _i, _i, _i, _i64, _p]),
     "bm_w8a8_sparse_f16_packed": (_i, [_p, _p, _p, _p, _p, _i, _i, _i, _i64, _p]),
+    "bm_f4_value_bytes": (_sz, [_i, _i]),
+    "bm_f4_scale_bytes": (_sz, [_i, _i, _i, _i]),
+    "bm_quantize_f4": (_i, [_p, _i, _p, _p, _p, _i, _i, _i64, _i, _i, _p]),
+    "bm_dequantize_f4": (_i, [_p, _p, _p, _p, _i, _i, _i, _i64, _i, _i, _p]),
+    "bm_f4_gemm": (_i, [_p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i64, _i, _p]),
     "bm_noalloc_last_device_status": (_i, [C.POINTER(_i)]),
     "bm_noalloc_selftest_bounded_wait": (_i, [C.c_uint, C.POINTER(_i)]),
     "bm_last_device_status": (_i, [C.POINTER(_i)]),
@@ -56,6 +61,9 @@ SIGNATURES = {
 
 BM_B_KN, BM_B_NK = 0, 1
 BM_META_REF, BM_META_ROWS, BM_META_TILED, BM_META_REF_F16, BM_META_ROWS_F16 = 0, 1, 2, 3, 4
+BM_F4_E8M0, BM_F4_E4M3 = 0, 1
+BM_SCALE_ROWS, BM_SCALE_TILED = 0, 1
+BM_F16, BM_BF16, BM_F32 = 0, 1, 2
 
 _lib = None
 

@@ -1,0 +1,270 @@
+// bm_f4.cu — extern "C" launchers of the 4-bit floating-point operators declared in include/bm_igemm.h.
+#include "host_common.cuh"
+#include "f4_gemm.cuh"
+#include "f4_gemm_few.cuh"
+#include "f4_quantize.cuh"
+
+namespace bm {
+
+static inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
+static inline int f4_row_bytes(int k) { return ceil_div(k, 32) * 16; }
+static inline int f4_tiles_k(int k, int fmt) { return ceil_div(k, 4 * f4_block(fmt)); }
+static inline int f4_scale_pitch(int k, int fmt) { return ceil_div(ceil_div(k, f4_block(fmt)), 16) * 16; }
+
+static int check_format(int format, int layout) {
+    if (format != BM_F4_E8M0 && format != BM_F4_E4M3) return fail_msg(BM_ERR_LAYOUT, "unknown 4-bit format tag");
+    if (layout != BM_SCALE_ROWS && layout != BM_SCALE_TILED) return fail_msg(BM_ERR_LAYOUT, "unknown scale layout tag");
+    return BM_OK;
+}
+static size_t f4_scale_bytes(int rows, int k, int fmt, int layout) {
+    return layout == BM_SCALE_TILED ? static_cast<size_t>(ceil_div(rows, 128)) * f4_tiles_k(k, fmt) * kF4TileBytes
+                                    : static_cast<size_t>(rows) * f4_scale_pitch(k, fmt);
+}
+static bool aligned_to(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+// ---- quantise ---------------------------------------------------------------------------
+template <int FMT, bool BF16>
+static int launch_quantize(const F4QuantParams& p, int sms, cudaStream_t stream) {
+    // Threads per row as in bm_quantize_rows_f16: four pieces a thread when there are many rows, one (two) when there are few.
+    auto group_for = [&](int held) { return ceil_div(ceil_div(p.pieces, held), 32) * 32; };
+    int held = 4, group = group_for(4);
+    if (p.rows <= sms) {
+        held = group_for(1) <= kF4QuantMaxThreads ? 1 : 2;
+        group = group_for(held);
+    }
+    const int most = held == 4 ? 512 : kF4QuantMaxThreads;
+    if (group > most) group = most;                                // the rest of such a row is read twice
+    const dim3 block(group, group == 32 ? 4 : 1);
+    const dim3 grid(ceil_div(p.rows_padded, static_cast<int>(block.y)));
+    if (held == 1) quantize_f4_kernel<FMT, BF16, 1><<<grid, block, 0, stream>>>(p);
+    else if (held == 2) quantize_f4_kernel<FMT, BF16, 2><<<grid, block, 0, stream>>>(p);
+    else quantize_f4_kernel<FMT, BF16, 4><<<grid, block, 0, stream>>>(p);
+    BM_CUDA_TRY(cudaGetLastError());
+    return BM_OK;
+}
+
+template <int FMT>
+static int launch_dequantize(const F4DequantParams& p, int type, int sms, cudaStream_t stream) {
+    const long long threads = static_cast<long long>(p.rows) * ceil_div(p.k, 8), blocks = (threads + 255) / 256;
+    const unsigned grid = static_cast<unsigned>(blocks < 64ll * sms ? blocks : 64ll * sms);
+    if (type == TYPE_F16) dequantize_f4_kernel<FMT, TYPE_F16><<<grid, 256, 0, stream>>>(p);
+    else if (type == TYPE_BF16) dequantize_f4_kernel<FMT, TYPE_BF16><<<grid, 256, 0, stream>>>(p);
+    else dequantize_f4_kernel<FMT, TYPE_F32><<<grid, 256, 0, stream>>>(p);
+    BM_CUDA_TRY(cudaGetLastError());
+    return BM_OK;
+}
+
+static int sm_count(int* sms) {                    // not current_device_state(): its first use allocates
+    int device = 0;
+    BM_CUDA_TRY(cudaGetDevice(&device));
+    BM_CUDA_TRY(cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, device));
+    return BM_OK;
+}
+
+// ---- product ----------------------------------------------------------------------------
+// tiled scales of `rows` rows as [row tile][4 * tiles_k][128 bytes], boxes of the scale tiles of one stage x `tiles` row tiles
+static int scale_map(CUtensorMap* map, const void* base, int rows, int k, int fmt, int tiles) {
+    const int tiles_k = f4_tiles_k(k, fmt);
+    const uint64_t dims[3] = {128, 4ull * tiles_k, static_cast<uint64_t>(ceil_div(rows, 128))};
+    const uint32_t box[3] = {128, 4u * f4_stage_tiles(fmt), static_cast<uint32_t>(tiles)};
+    return cached_tensor_map(map, base, 3, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, dims, 128, box, CU_TENSOR_MAP_SWIZZLE_NONE, true,
+                             static_cast<uint64_t>(tiles_k) * kF4TileBytes);
+}
+
+struct F4Operands {
+    const uint8_t *a, *sa, *b, *sb;
+    int fmt, type, M, N, K;
+};
+
+template <bool PAIR, int FMT, int TYPE>
+static int launch_f4_inst(const F4Operands& o, F4GemmParams& p, DeviceState* dev, cudaStream_t stream) {
+    using Cfg = F4Cfg<PAIR, FMT>;
+    const size_t elem = TYPE == TYPE_F32 ? 4 : 2;
+    const int pitch = f4_row_bytes(o.K);
+    CUtensorMap ma, msa, mb, msb, mo;
+    if (int rc = make_tensor_map_u8(&ma, o.a, pitch, o.M, pitch, 128, 128, true)) return rc;
+    if (int rc = make_tensor_map_u8(&mb, o.b, pitch, o.N, pitch, 128, 128, true)) return rc;
+    if (int rc = scale_map(&msa, o.sa, o.M, o.K, FMT, 1)) return rc;
+    if (int rc = scale_map(&msb, o.sb, o.N, o.K, FMT, Cfg::BN / 128)) return rc;
+    mo = ma;                                         // placeholder unless the output qualifies for TMA stores
+    if (aligned16(p.out) && (static_cast<size_t>(p.ld) * elem) % 16 == 0 && opt(OPT_TMA_STORE) != 0) {
+        if (int rc = make_tensor_map_out(&mo, p.out, o.N, o.M, static_cast<size_t>(p.ld) * elem, static_cast<int>(elem))) return rc;
+        p.tma_ok = 1;
+    }
+    p.tiles_m = ceil_div(o.M, Cfg::ROWS);
+    p.tiles_n = ceil_div(o.N, Cfg::BN);
+    p.k_blocks = ceil_div(o.K, kF4BK);
+    p.status = dev->status;
+    const long long tiles = static_cast<long long>(p.tiles_m) * p.tiles_n;
+    if (tiles > 0x7FFFFFFF) return fail_msg(BM_ERR_TOO_LARGE, "more than 2^31 output tiles");
+    const int slots = PAIR ? dev->sm_count / 2 : dev->sm_count;
+    const int units = tiles < slots ? static_cast<int>(tiles) : slots;
+    if (PAIR) p.group_m = p.tiles_m >= 2 * p.tiles_n && p.tiles_m >= 16 ? 8 : 0;      // as for the int8 pair kernel
+    auto kern = f4_gemm_kernel<PAIR, FMT, TYPE>;
+    static ConfiguredFlags flags;
+    if (int rc = ensure_smem_limit(flags, kern, Cfg::SMEM_BYTES)) return rc;
+    BM_CUDA_TRY(launch_pdl(kern, dim3(PAIR ? 2 * units : units), dim3(kDenseThreads), Cfg::SMEM_BYTES, stream, PAIR ? 2 : 1, ma, msa, mb,
+                           msb, mo, p));
+    return BM_OK;
+}
+template <bool PAIR>
+static int launch_f4(const F4Operands& o, F4GemmParams& p, DeviceState* dev, cudaStream_t stream) {
+#define BM_F4_CASE(F, T) if (o.fmt == F && o.type == T) return launch_f4_inst<PAIR, F, T>(o, p, dev, stream)
+    BM_F4_CASE(FMT_E8M0, TYPE_F16); BM_F4_CASE(FMT_E8M0, TYPE_BF16); BM_F4_CASE(FMT_E8M0, TYPE_F32);
+    BM_F4_CASE(FMT_E4M3, TYPE_F16); BM_F4_CASE(FMT_E4M3, TYPE_BF16); BM_F4_CASE(FMT_E4M3, TYPE_F32);
+#undef BM_F4_CASE
+    return fail_msg(BM_ERR_LAYOUT, "unknown element type tag");
+}
+
+template <int FMT, int TYPE>
+static int launch_f4_few(const CUtensorMap& mw, const CUtensorMap& msw, const CUtensorMap& mx, const CUtensorMap& msx, const F4FewParams& p,
+                         int tiles, cudaStream_t stream) {
+    auto kern = f4_gemm_few_kernel<FMT, TYPE>;
+    static ConfiguredFlags flags;
+    if (int rc = ensure_smem_limit(flags, kern, kF4FewSmemBytes)) return rc;
+    BM_CUDA_TRY(launch_pdl(kern, dim3(tiles * p.split), dim3(kF4FewThreads), kF4FewSmemBytes, stream, p.split, mw, msw, mx, msx, p));
+    return BM_OK;
+}
+
+static int f4_few(const F4Operands& o, const F4GemmParams& g, DeviceState* dev, cudaStream_t stream) {
+    F4FewParams p{};
+    p.out = g.out;
+    p.ld = g.ld;
+    p.tokens = o.M;
+    p.channels = o.N;
+    p.token_scale = g.row_scale;
+    p.channel_scale = g.col_scale;
+    p.tokens_padded = ceil_div(o.M, 16) * 16;
+    p.k_blocks = ceil_div(o.K, kF4BK);
+    p.status = dev->status;
+    const int stage_bytes = 128 * 128 + p.tokens_padded * 128 + 2 * f4_stage_tiles(o.fmt) * kF4TileBytes;
+    p.stages = kF4FewRingBytes / stage_bytes;
+    if (p.stages > kF4FewMaxStages) p.stages = kF4FewMaxStages;
+    p.tmem_cols = 32;
+    while (p.tmem_cols < p.tokens_padded + 2 * f4_stage_tiles(o.fmt) * 4) p.tmem_cols *= 2;
+    const int tiles = ceil_div(o.N, 128);
+    p.split = 1;
+    while (p.split < 8 && 2 * p.split * tiles <= 2 * dev->sm_count && 2 * p.split <= p.k_blocks) p.split *= 2;
+    CUtensorMap mw, msw, mx, msx;
+    const int pitch = f4_row_bytes(o.K);
+    if (int rc = make_tensor_map_u8(&mw, o.b, pitch, o.N, pitch, 128, 128, true)) return rc;
+    if (int rc = make_tensor_map_u8(&mx, o.a, pitch, o.M, pitch, 128, p.tokens_padded, true)) return rc;
+    if (int rc = scale_map(&msw, o.sb, o.N, o.K, o.fmt, 1)) return rc;
+    if (int rc = scale_map(&msx, o.sa, o.M, o.K, o.fmt, 1)) return rc;
+#define BM_F4_CASE(F, T) if (o.fmt == F && o.type == T) return launch_f4_few<F, T>(mw, msw, mx, msx, p, tiles, stream)
+    BM_F4_CASE(FMT_E8M0, TYPE_F16); BM_F4_CASE(FMT_E8M0, TYPE_BF16); BM_F4_CASE(FMT_E8M0, TYPE_F32);
+    BM_F4_CASE(FMT_E4M3, TYPE_F16); BM_F4_CASE(FMT_E4M3, TYPE_BF16); BM_F4_CASE(FMT_E4M3, TYPE_F32);
+#undef BM_F4_CASE
+    return fail_msg(BM_ERR_LAYOUT, "unknown element type tag");
+}
+
+}  // namespace bm
+
+using namespace bm;
+
+extern "C" {
+
+size_t bm_f4_value_bytes(int R, int K) {
+    return R <= 0 || K <= 0 ? 0 : static_cast<size_t>(R) * f4_row_bytes(K);
+}
+
+size_t bm_f4_scale_bytes(int R, int K, int format, int scale_layout) {
+    if (R <= 0 || K <= 0 || check_format(format, scale_layout) != BM_OK) return 0;
+    return f4_scale_bytes(R, K, format, scale_layout);
+}
+
+int bm_quantize_f4(const void* X, int x_type, uint8_t* Q, uint8_t* S, float* row_scale, int R, int K, int64_t ldx, int format,
+                   int scale_layout, void* stream) {
+    if (!X || !Q || !S) return fail_msg(BM_ERR_NULL, "pointer is NULL");
+    if (int rc = check_format(format, scale_layout)) return rc;
+    if (x_type != BM_F16 && x_type != BM_BF16) return fail_msg(BM_ERR_LAYOUT, "X must be fp16 or bf16");
+    if (format == BM_F4_E4M3 && !row_scale) return fail_msg(BM_ERR_NULL, "the E4M3 format needs row_scale");
+    if (R <= 0 || K <= 0 || K > 0x7FFFFC00 || R > 0x7FFFFF00) return fail_msg(BM_ERR_SHAPE, "R and K must be positive and below 2^31 - 1024");
+    if (ldx < K) return fail_msg(BM_ERR_SHAPE, "row pitch is smaller than the row length");
+    if (!aligned16(Q) || !aligned16(S) || !aligned_to(X, 2) || !aligned_to(row_scale, 4))
+        return fail_msg(BM_ERR_ALIGN, "Q and S must be 16-byte aligned, X and row_scale to their elements");
+    int sms = 0;
+    if (int rc = sm_count(&sms)) return rc;
+    F4QuantParams p{};
+    p.x = static_cast<const uint16_t*>(X);
+    p.ldx = ldx;
+    p.q = Q;
+    p.s = S;
+    p.row_scale = row_scale;
+    p.rows = R;
+    p.k = K;
+    p.k_padded = 2 * f4_row_bytes(K);
+    const int share = f4_block(format) / 8;
+    if (scale_layout == BM_SCALE_TILED) {
+        p.tiles_k = f4_tiles_k(K, format);
+        p.pieces = p.tiles_k * 4 * share;
+        p.rows_padded = ceil_div(R, 128) * 128;
+    } else {
+        p.scale_pitch = f4_scale_pitch(K, format);
+        p.pieces = p.scale_pitch * share;
+        p.rows_padded = R;
+    }
+    p.vec_ok = aligned16(X) && ldx % 8 == 0;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (format == BM_F4_E8M0) return x_type == BM_BF16 ? launch_quantize<FMT_E8M0, true>(p, sms, st) : launch_quantize<FMT_E8M0, false>(p, sms, st);
+    return x_type == BM_BF16 ? launch_quantize<FMT_E4M3, true>(p, sms, st) : launch_quantize<FMT_E4M3, false>(p, sms, st);
+}
+
+int bm_dequantize_f4(const uint8_t* Q, const uint8_t* S, const float* row_scale, void* out, int out_type, int R, int K, int64_t ldo,
+                     int format, int scale_layout, void* stream) {
+    if (!Q || !S || !out) return fail_msg(BM_ERR_NULL, "pointer is NULL");
+    if (int rc = check_format(format, scale_layout)) return rc;
+    if (out_type != BM_F16 && out_type != BM_BF16 && out_type != BM_F32) return fail_msg(BM_ERR_LAYOUT, "unknown element type tag");
+    if (R <= 0 || K <= 0 || K > 0x7FFFFC00 || R > 0x7FFFFF00) return fail_msg(BM_ERR_SHAPE, "R and K must be positive and below 2^31 - 1024");
+    if (ldo < K) return fail_msg(BM_ERR_SHAPE, "row pitch is smaller than the row length");
+    const size_t elem = out_type == BM_F32 ? 4 : 2;
+    if (!aligned16(Q) || !aligned16(S) || !aligned_to(out, elem) || !aligned_to(row_scale, 4))
+        return fail_msg(BM_ERR_ALIGN, "Q and S must be 16-byte aligned, the output and row_scale to their elements");
+    int sms = 0;
+    if (int rc = sm_count(&sms)) return rc;
+    F4DequantParams p{};
+    p.q = Q;
+    p.s = S;
+    p.row_scale = row_scale;
+    p.out = out;
+    p.ldo = ldo;
+    p.rows = R;
+    p.k = K;
+    p.k_padded = 2 * f4_row_bytes(K);
+    if (scale_layout == BM_SCALE_TILED) p.tiles_k = f4_tiles_k(K, format);
+    else p.scale_pitch = f4_scale_pitch(K, format);
+    p.vec_ok = aligned16(out) && (static_cast<size_t>(ldo) * elem) % 16 == 0;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    return format == BM_F4_E8M0 ? launch_dequantize<FMT_E8M0>(p, out_type, sms, st) : launch_dequantize<FMT_E4M3>(p, out_type, sms, st);
+}
+
+int bm_f4_gemm(const uint8_t* A, const uint8_t* SA, const float* ra, const uint8_t* W, const uint8_t* SW, const float* rw, void* D,
+               int d_type, int M, int N, int K, int64_t ldd, int format, void* stream) {
+    if (!A || !SA || !W || !SW || !D) return fail_msg(BM_ERR_NULL, "pointer is NULL");
+    if (int rc = check_format(format, BM_SCALE_TILED)) return rc;
+    if (d_type != BM_F16 && d_type != BM_BF16 && d_type != BM_F32) return fail_msg(BM_ERR_LAYOUT, "unknown element type tag");
+    if (M <= 0 || N <= 0 || K <= 0 || K > 0x7FFFFC00 || M > 0x7FFFFF00 || N > 0x7FFFFF00)
+        return fail_msg(BM_ERR_SHAPE, "M, N, K must be positive and below 2^31 - 1024");
+    if (ldd < N) return fail_msg(BM_ERR_SHAPE, "output pitch is smaller than the row length");
+    if (!aligned16(A) || !aligned16(SA) || !aligned16(W) || !aligned16(SW)) return fail_msg(BM_ERR_ALIGN, "operands and scales must be 16-byte aligned");
+    if (!aligned_to(D, d_type == BM_F32 ? 4 : 2) || !aligned_to(ra, 4) || !aligned_to(rw, 4))
+        return fail_msg(BM_ERR_ALIGN, "output and factors must be aligned to their elements");
+    DeviceState* dev = nullptr;
+    if (int rc = current_device_state(&dev)) return rc;
+    F4Operands o{A, SA, W, SW, format, d_type, M, N, K};
+    F4GemmParams p{};
+    p.out = D;
+    p.ld = ldd;
+    p.rows = M;
+    p.cols = N;
+    p.row_scale = ra;
+    p.col_scale = rw;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const int forced = opt(OPT_F4_KERNEL);
+    if (M <= kF4FewMaxTokens && (forced == 1 || (forced == 0 && M <= 64))) return f4_few(o, p, dev, st);
+    const long long pair_tiles = static_cast<long long>(ceil_div(M, 256)) * ceil_div(N, 256);
+    const bool pair = dev->sm_count >= 2 && (forced == 3 || (forced != 2 && pair_tiles > dev->sm_count / 4));
+    return pair ? launch_f4<true>(o, p, dev, st) : launch_f4<false>(o, p, dev, st);
+}
+
+}  // extern "C"

@@ -54,6 +54,7 @@ enum : int {
     OPT_GATHER_GBS,          // fused all-gather: GB/s of peer stores a GPU may send (0 = unpaced)
     OPT_DENSE_DECODE,        // few tokens: -1 automatic, 0 never, 1 always the channels-on-lanes kernel (where it applies)
     OPT_DECODE_TILE_ROWS,    // row-balanced decode tiles: rows per ring stage (0 automatic; 32 / 64 / 128 pins it)
+    OPT_F4_KERNEL,           // 4-bit GEMM: 0 choose, 1 few tokens (where it applies), 2 tiles of 128 x 128, 3 CTA pairs
     OPT_COUNT
 };
 struct OptionSpec { const char* name; const char* env; int def; };
@@ -65,6 +66,7 @@ inline const OptionSpec* option_specs() {
         {"sparse_col_first", "BM_SPARSE_COL_FIRST", -1}, {"tail_narrow", "BM_TAIL_NARROW", 1},
         {"pdl", "BM_PDL", 1},                     {"gather_gbs", "BM_GATHER_GBS", 680},
         {"dense_decode", "BM_DENSE_DECODE", -1},  {"decode_tile_rows", "BM_DECODE_TILE_ROWS", 0},
+        {"f4_kernel", "BM_F4_KERNEL", 0},
     };
     return specs;
 }
@@ -183,18 +185,18 @@ inline EncodeTiledFn encode_tiled_fn() {
 // to ten times per launch.  The cache is bounded: when it is full it is emptied and refilled.
 struct MapKey {
     const void* base;
-    uint64_t d0, d1, d2, pitch;
+    uint64_t d0, d1, d2, pitch, pitch2;
     uint32_t b0, b1, b2, kind;           // kind: element size | swizzle << 8 | rank << 16 | L2 promotion << 24
     bool operator==(const MapKey& o) const {
-        return base == o.base && d0 == o.d0 && d1 == o.d1 && d2 == o.d2 && pitch == o.pitch && b0 == o.b0 &&
-               b1 == o.b1 && b2 == o.b2 && kind == o.kind;
+        return base == o.base && d0 == o.d0 && d1 == o.d1 && d2 == o.d2 && pitch == o.pitch &&
+               pitch2 == o.pitch2 && b0 == o.b0 && b1 == o.b1 && b2 == o.b2 && kind == o.kind;
     }
 };
 struct MapKeyHash {
     size_t operator()(const MapKey& k) const {
         uint64_t h = reinterpret_cast<uintptr_t>(k.base) * 0x9E3779B97F4A7C15ull;
         auto mix = [&h](uint64_t v) { h = (h ^ v) * 0x100000001B3ull; h ^= h >> 29; };
-        mix(k.d0); mix(k.d1); mix(k.d2); mix(k.pitch);
+        mix(k.d0); mix(k.d1); mix(k.d2); mix(k.pitch); mix(k.pitch2);
         mix((static_cast<uint64_t>(k.b0) << 32) | k.b1);
         mix((static_cast<uint64_t>(k.b2) << 32) | k.kind);
         return static_cast<size_t>(h);
@@ -212,13 +214,13 @@ inline MapCache& map_cache() {
 }
 
 // Encodes (or fetches) a tiled map of rank 2 or 3.  dims / box are innermost first; `pitch` is the byte
-// stride of dimension 1; dimension 2 of a rank-3 map steps by 128 bytes (K blocks of a row-major operand).
+// stride of dimension 1, `pitch2` of dimension 2 of a rank-3 map (128: K blocks of a row-major operand).
 inline int cached_tensor_map(CUtensorMap* map, const void* base, int rank, CUtensorMapDataType type, int elem_size,
                              const uint64_t (&dims)[3], uint64_t pitch, const uint32_t (&box)[3],
-                             CUtensorMapSwizzle swizzle, bool l2_promote) {
+                             CUtensorMapSwizzle swizzle, bool l2_promote, uint64_t pitch2 = 128) {
     EncodeTiledFn fn = encode_tiled_fn();
     if (!fn) return fail_msg(BM_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
-    MapKey key{base, dims[0], dims[1], rank == 3 ? dims[2] : 0, pitch, box[0], box[1], rank == 3 ? box[2] : 0,
+    MapKey key{base, dims[0], dims[1], rank == 3 ? dims[2] : 0, pitch, rank == 3 ? pitch2 : 0, box[0], box[1], rank == 3 ? box[2] : 0,
                static_cast<uint32_t>(elem_size) | (static_cast<uint32_t>(swizzle) << 8) | (static_cast<uint32_t>(rank) << 16) |
                    (l2_promote ? 1u << 24 : 0u)};
     MapCache& cache = map_cache();
@@ -232,7 +234,7 @@ inline int cached_tensor_map(CUtensorMap* map, const void* base, int rank, CUten
         }
     }
     cuuint64_t gdims[3] = {dims[0], dims[1], dims[2]};
-    cuuint64_t strides[2] = {pitch, 128};
+    cuuint64_t strides[2] = {pitch, pitch2};
     cuuint32_t gbox[3] = {box[0], box[1], box[2]};
     cuuint32_t elem_strides[3] = {1, 1, 1};
     CUresult r = fn(map, type, static_cast<cuuint32_t>(rank), const_cast<void*>(base), gdims, strides, gbox, elem_strides,

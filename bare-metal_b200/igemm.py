@@ -13,13 +13,14 @@ Reference symbol                              -> function here
   igemm_persistent                            -> igemm_persistent (tile counter ignored)
   igemm_pipelined_cpasync_perchannel          -> igemm_pipelined_cpasync_perchannel
   igemm_sparse_tiled (+ _persistent)          -> igemm_sparse_tiled
-plus the entry points the B200 workloads add: igemm_i32, w8a8_linear, sparse weights.
+plus the entry points the B200 workloads add: igemm_i32, w8a8_linear, sparse weights, 4-bit floating point.
 """
 from __future__ import annotations
 
 import torch
 
 from . import _lib
+from ._lib import BM_BF16, BM_F16, BM_F32, BM_F4_E4M3, BM_F4_E8M0, BM_SCALE_ROWS, BM_SCALE_TILED  # noqa: F401
 from ._lib import BM_B_KN, BM_B_NK, BM_META_REF, BM_META_REF_F16, BM_META_ROWS, BM_META_ROWS_F16, BM_META_TILED, BmError  # noqa: F401
 
 
@@ -292,6 +293,89 @@ def w8a8_sparse_linear_packed(X, W_packed, D, sa, sw, M, N, K, ldd=None):
                                      _dev(sa, torch.float32, "sa"), _dev(sw, torch.float32, "sw"), M, N, K, ldd,
                                      _stream())
     _lib.check(rc, "bm_w8a8_sparse_f16_packed")
+    return D
+
+
+# --------------------------------------------------------------------------------------
+# 4-bit floating point: E2M1 values with one scale per block (formats and layouts: include/bm_igemm.h)
+# --------------------------------------------------------------------------------------
+_ELEMENT = {torch.float16: BM_F16, torch.bfloat16: BM_BF16, torch.float32: BM_F32}
+_F4_BLOCK = {BM_F4_E8M0: 32, BM_F4_E4M3: 16}
+
+
+def _here(t: torch.Tensor, name: str) -> torch.Tensor:
+    """A CUDA tensor of the current device (kernels run on its current stream)."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise BmError(f"{name} must be a CUDA tensor")
+    if t.get_device() != torch.cuda.current_device():
+        raise BmError(f"{name} must be on the current device")
+    return t
+
+
+def _buffer(t: torch.Tensor, dtype, numel: int, name: str) -> int:
+    if _here(t, name).dtype != dtype:
+        raise BmError(f"{name} must have dtype {dtype}, got {t.dtype}")
+    if not t.is_contiguous() or t.numel() < numel:
+        raise BmError(f"{name} must be contiguous and hold {numel} elements")
+    return t.data_ptr()
+
+
+def _f4_rows(t: torch.Tensor, name: str) -> int:
+    """Elements between the rows of a matrix whose rows are contiguous."""
+    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise BmError(f"{name} must be a matrix with unit stride along its rows")
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _f4_matrix(q, s, r, R, K, fmt, layout, name):
+    """Pointers of the three parts of a 4-bit matrix."""
+    if fmt not in _F4_BLOCK:
+        raise BmError(f"unknown 4-bit format tag {fmt}")
+    L = _lib.load()
+    return (_buffer(q, torch.uint8, L.bm_f4_value_bytes(R, K), f"{name} values"),
+            _buffer(s, torch.uint8, L.bm_f4_scale_bytes(R, K, fmt, layout), f"{name} scales"),
+            None if r is None else _buffer(r, torch.float32, R, f"{name} row factors"))
+
+
+def quantize_f4(X, fmt=BM_F4_E4M3, scale_layout=BM_SCALE_TILED):
+    """Rows of a fp16 / bf16 matrix to 4 bits: (values uint8 [R, ceil(K/32)*16], scales uint8 — [R, pitch] in rows, 1-D tiled —,
+    row factors fp32 [R], None for BM_F4_E8M0)."""
+    L = _lib.load()
+    if _here(X, "X").dtype not in (torch.float16, torch.bfloat16):
+        raise BmError("X must be float16 or bfloat16")
+    ldx = _f4_rows(X, "X")
+    R, K = X.shape
+    nbytes = L.bm_f4_scale_bytes(R, K, fmt, scale_layout)
+    q = torch.empty((R, (K + 31) // 32 * 16), dtype=torch.uint8, device=X.device)
+    s = torch.empty((R, nbytes // R) if scale_layout == BM_SCALE_ROWS and R else nbytes, dtype=torch.uint8, device=X.device)
+    r = torch.empty(R, dtype=torch.float32, device=X.device) if fmt == BM_F4_E4M3 else None
+    _lib.check(L.bm_quantize_f4(X.data_ptr(), _ELEMENT[X.dtype], q.data_ptr(), s.data_ptr(), None if r is None else r.data_ptr(),
+                                R, K, ldx, fmt, scale_layout, _stream()), "bm_quantize_f4")
+    return q, s, r
+
+
+def dequantize_f4(q, s, r, R, K, dtype=torch.float16, fmt=BM_F4_E4M3, scale_layout=BM_SCALE_TILED, out=None):
+    """The numbers of a 4-bit matrix as [R, K] fp16, bf16 or fp32."""
+    if out is None:
+        out = torch.empty((R, K), dtype=dtype, device=q.device)
+    elif _here(out, "out").dtype not in _ELEMENT or tuple(out.shape) != (R, K):
+        raise BmError(f"out must be a floating-point matrix [{R}, {K}]")
+    if out.dtype not in _ELEMENT:
+        raise BmError(f"the output cannot have dtype {out.dtype}")
+    rc = _lib.load().bm_dequantize_f4(*_f4_matrix(q, s, r, R, K, fmt, scale_layout, "Q"), out.data_ptr(), _ELEMENT[out.dtype], R, K,
+                                      _f4_rows(out, "out"), fmt, scale_layout, _stream())
+    _lib.check(rc, "bm_dequantize_f4")
+    return out
+
+
+def f4_linear(Xq, Xs, Xr, Wq, Ws, Wr, D, M, N, K, fmt=BM_F4_E4M3):
+    """D[M,N] = X W^T of two 4-bit matrices with tiled scales (X[M,K], W[N,K]; row factors may be None); D fp16, bf16 or fp32."""
+    if _here(D, "D").dtype not in _ELEMENT or tuple(D.shape) != (M, N):
+        raise BmError(f"D must be a floating-point matrix [{M}, {N}]")
+    x = _f4_matrix(Xq, Xs, Xr, M, K, fmt, BM_SCALE_TILED, "X")
+    w = _f4_matrix(Wq, Ws, Wr, N, K, fmt, BM_SCALE_TILED, "W")
+    rc = _lib.load().bm_f4_gemm(*x, *w, D.data_ptr(), _ELEMENT[D.dtype], M, N, K, _f4_rows(D, "D"), fmt, _stream())
+    _lib.check(rc, "bm_f4_gemm")
     return D
 
 

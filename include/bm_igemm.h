@@ -242,6 +242,51 @@ int bm_w8a8_sparse_f16_packed(const int8_t *X, const void *W_packed, uint16_t *D
                               const float *sw_n, int M, int N, int K, int64_t ldd, void *stream);
 
 /* =======================================================================================
+ * 4-bit floating point (no counterpart in the reference): E2M1 values with one scale per block along a row.
+ *
+ *   BM_F4_E8M0  blocks of 32, scale 2^(byte - 127) (byte 255: NaN) — the OCP Microscaling format MXFP4
+ *   BM_F4_E4M3  blocks of 16, the scale an E4M3 number, and one fp32 factor per row
+ *
+ * A matrix of R rows and K columns is
+ *   values  [R x ceil(K/32)*16 bytes]: two to a byte, the lower column in the low four bits, zeros beyond K;
+ *   scales  BM_SCALE_ROWS: [R x pitch] bytes, pitch = the blocks of a row rounded up to 16, zeros behind them; or
+ *           BM_SCALE_TILED: tiles of 128 rows x 4 blocks, 512 bytes each, ceil(blocks/4) tiles for each 128 rows: the byte of
+ *           row r and block g at ((r/128)*ceil(blocks/4) + g/4)*512 + (r%32)*16 + (r%128)/32*4 + g%4; zeros
+ *           in rows and blocks beyond the matrix — what the product reads;
+ *   row_scale [R] fp32 (BM_F4_E4M3; a power of two when bm_quantize_f4 wrote it).
+ * ===================================================================================== */
+#define BM_F4_E8M0    0
+#define BM_F4_E4M3    1
+#define BM_SCALE_ROWS  0
+#define BM_SCALE_TILED 1
+/* element types of 16- and 32-bit operands */
+#define BM_F16  0   /* IEEE binary16 */
+#define BM_BF16 1   /* bfloat16      */
+#define BM_F32  2   /* IEEE binary32 */
+
+/* bytes of the values and of the scales of an R x K matrix (0 for bad arguments) */
+size_t bm_f4_value_bytes(int R, int K);
+size_t bm_f4_scale_bytes(int R, int K, int format, int scale_layout);
+
+/* Rows of X[R x K] (BM_F16 or BM_BF16, `ldx` elements between rows) to 4 bits.  With amax the largest |x| of a block and
+ * top that of its row, infinities and NaNs left out:
+ *   BM_F4_E8M0  s = 2^(floor(log2 amax) - 2), q = E2M1(x / s)
+ *   BM_F4_E4M3  t = row_scale = 2^(floor(log2 top) - 10) (1 for a row of zeros), s = E4M3(amax / (6 t)), q = E2M1(x / (t s))
+ * each rounded once to the nearest, ties to even, q saturating at 6 (exponents are held within their types' range).  A block
+ * with an infinity or a NaN gets the scale NaN and the values 0.  row_scale may be NULL for BM_F4_E8M0.
+ * Q and S 16-byte aligned; any K, any ldx >= K. */
+int bm_quantize_f4(const void *X, int x_type, uint8_t *Q, uint8_t *S, float *row_scale, int R, int K, int64_t ldx,
+                   int format, int scale_layout, void *stream);
+/* Back to numbers: out[r][k] = value * scale * row_scale[r] (row_scale NULL: 1), rounded once to `out_type`. */
+int bm_dequantize_f4(const uint8_t *Q, const uint8_t *S, const float *row_scale, void *out, int out_type, int R, int K,
+                     int64_t ldo, int format, int scale_layout, void *stream);
+
+/* D[m][n] = (sum_k A[m][k] * W[n][k], both times their scales, added in fp32) * (ra[m] * rw[n]), rounded once to
+ * `d_type`.  A[M x K] and W[N x K] in `format` with BM_SCALE_TILED scales; ra, rw: row factors, NULL for ones. */
+int bm_f4_gemm(const uint8_t *A, const uint8_t *SA, const float *ra, const uint8_t *W, const uint8_t *SW, const float *rw,
+               void *D, int d_type, int M, int N, int K, int64_t ldd, int format, void *stream);
+
+/* =======================================================================================
  * Library state
  * ===================================================================================== */
 /* Reads (and clears) the device status word that a bounded in-kernel wait sets when it gives
@@ -257,7 +302,8 @@ int bm_last_device_status(int *code);
  * "dense_decode" (dense weights [N x K], at most 256 tokens: -1 choose, 0 never / 1 always the kernel with
  * channels on the lanes),
  * "decode_tile_rows" (row-balanced decode tiles on packed weights: 0 = choose the ring-stage height
- * from the rows a CTA is dealt, 32 / 64 / 128 pins it).
+ * from the rows a CTA is dealt, 32 / 64 / 128 pins it),
+ * "f4_kernel" (4-bit GEMM: 0 = choose, 1 the few-token kernel where M <= 128, 2 tiles of 128 x 128, 3 CTA pairs).
  * Each starts from the environment variable BM_<NAME> read once at first use, else its default;
  * launchers never read the environment on the launch path.  Process-wide; set them while no
  * other thread is launching.  Unknown names return BM_ERR_LAYOUT. */
