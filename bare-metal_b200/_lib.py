@@ -47,6 +47,8 @@ SIGNATURES = {
     "bm_quantize_f4": (_i, [_p, _i, _p, _p, _p, _i, _i, _i64, _i, _i, _p]),
     "bm_dequantize_f4": (_i, [_p, _p, _p, _p, _i, _i, _i, _i64, _i, _i, _p]),
     "bm_f4_gemm": (_i, [_p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i64, _i, _p]),
+    "bm_moe_f4_workspace_bytes": (_sz, [_i, _i, _i, _i, _i]),
+    "bm_moe_f4": (_i, [_p, _p, _i] + [_p] * 9 + [_i] * 5 + [_i64, _i64, _i, _i, _p, _sz, _p]),
     "bm_noalloc_last_device_status": (_i, [C.POINTER(_i)]),
     "bm_noalloc_selftest_bounded_wait": (_i, [C.c_uint, C.POINTER(_i)]),
     "bm_last_device_status": (_i, [C.POINTER(_i)]),

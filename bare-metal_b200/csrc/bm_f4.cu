@@ -2,6 +2,7 @@
 #include "host_common.cuh"
 #include "f4_gemm.cuh"
 #include "f4_gemm_few.cuh"
+#include "f4_moe.cuh"
 #include "f4_quantize.cuh"
 
 namespace bm {
@@ -158,6 +159,61 @@ static int f4_few(const F4Operands& o, const F4GemmParams& g, DeviceState* dev, 
     return fail_msg(BM_ERR_LAYOUT, "unknown element type tag");
 }
 
+// ---- expert layer -----------------------------------------------------------------------
+static MoeWorkspace moe_workspace(int T, int H, int I, int E, int top) {
+    auto up = [](size_t v) { return (v + 255) & ~static_cast<size_t>(255); };
+    MoeWorkspace w{};
+    const size_t a = static_cast<size_t>(T) * top;
+    w.counter_words = E + 4 + static_cast<int>(a);
+    w.h_pitch = ceil_div(I, 32) * 32;
+    w.y_pitch = ceil_div(H, 32) * 32;
+    w.counters = 0;
+    w.x_scale = w.counters + up(4ull * w.counter_words);
+    w.ids = w.x_scale + up(4ull * T);
+    w.weights = w.ids + up(4ull * a);
+    w.h = w.weights + up(4ull * a);
+    w.y = w.h + up(4ull * a * w.h_pitch);
+    w.bytes = w.y + up(4ull * a * w.y_pitch);
+    return w;
+}
+static bool moe_in_range(int T, int H, int I, int E, int top) {
+    return T > 0 && T <= kMoeMaxTokens && E > 0 && E <= kMoeMaxExperts && top > 0 && top <= kMoeMaxTop && top <= E && H > 0 && H <= kMoeMaxDim &&
+           I > 0 && I <= kMoeMaxDim;
+}
+
+// expert matrices [outer][rows][K]: boxes of 16 rows, as box_outer x (16 / box_outer)
+static int expert_maps(CUtensorMap* values, CUtensorMap* scales, const uint8_t* q, const uint8_t* s, int outer, int rows, int k, int fmt,
+                       uint32_t box_outer) {
+    const uint64_t pitch = f4_row_bytes(k), s_pitch = f4_scale_pitch(k, fmt);
+    const uint64_t dims[3] = {pitch, static_cast<uint64_t>(rows), static_cast<uint64_t>(outer)};
+    const uint64_t s_dims[3] = {s_pitch, static_cast<uint64_t>(rows), static_cast<uint64_t>(outer)};
+    const uint32_t box[3] = {128, 16 / box_outer, box_outer}, s_box[3] = {16, 16 / box_outer, box_outer};
+    if (int rc = cached_tensor_map(values, q, 3, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, dims, pitch, box, CU_TENSOR_MAP_SWIZZLE_128B, true, pitch * rows))
+        return rc;
+    return cached_tensor_map(scales, s, 3, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, s_dims, s_pitch, s_box, CU_TENSOR_MAP_SWIZZLE_NONE, true, s_pitch * rows);
+}
+
+template <int FMT, bool BF16>
+static int launch_moe(const CUtensorMap& w13, const CUtensorMap& s13, const CUtensorMap& w2, const CUtensorMap& s2, const MoeParams& p,
+                      int clusters, int ctas, cudaStream_t stream) {
+    auto kern = moe_experts_kernel<FMT, BF16>;
+    static ConfiguredFlags flags;
+    if (int rc = ensure_smem_limit(flags, kern, kMoeSmemBytes)) return rc;
+    BM_CUDA_TRY(launch_pdl(moe_router_kernel<BF16>, dim3(clusters * kMoeRouterCtas), dim3(kMoeRouterThreads), 0, stream, kMoeRouterCtas, p));
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(ctas);
+    cfg.blockDim = dim3(kMoeThreads);
+    cfg.dynamicSmemBytes = kMoeSmemBytes;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeCooperative;             // its CTAs wait for one another
+    attr[0].val.cooperative = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    BM_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, w13, s13, w2, s2, p));
+    return BM_OK;
+}
+
 }  // namespace bm
 
 using namespace bm;
@@ -265,6 +321,75 @@ int bm_f4_gemm(const uint8_t* A, const uint8_t* SA, const float* ra, const uint8
     const long long pair_tiles = static_cast<long long>(ceil_div(M, 256)) * ceil_div(N, 256);
     const bool pair = dev->sm_count >= 2 && (forced == 3 || (forced != 2 && pair_tiles > dev->sm_count / 4));
     return pair ? launch_f4<true>(o, p, dev, st) : launch_f4<false>(o, p, dev, st);
+}
+
+size_t bm_moe_f4_workspace_bytes(int T, int H, int I, int E, int top) {
+    return moe_in_range(T, H, I, E, top) ? moe_workspace(T, H, I, E, top).bytes : 0;
+}
+
+int bm_moe_f4(const void* X, const void* router, int x_type, const uint8_t* W13, const uint8_t* S13, const float* r13, const uint8_t* W2,
+              const uint8_t* S2, const float* r2, void* Y, int32_t* ids, float* weights, int T, int H, int I, int E, int top, int64_t ldx,
+              int64_t ldy, int format, int normalize, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!X || !router || !W13 || !S13 || !W2 || !S2 || !Y || !workspace) return fail_msg(BM_ERR_NULL, "pointer is NULL");
+    if (int rc = check_format(format, BM_SCALE_ROWS)) return rc;
+    if (x_type != BM_F16 && x_type != BM_BF16) return fail_msg(BM_ERR_LAYOUT, "activations must be fp16 or bf16");
+    if (T <= 0 || H <= 0 || I <= 0 || E <= 0 || top <= 0 || top > E) return fail_msg(BM_ERR_SHAPE, "T, H, I, E must be positive, 1 <= top <= E");
+    if (!moe_in_range(T, H, I, E, top)) return fail_msg(BM_ERR_TOO_LARGE, "at most 64 tokens, 256 experts, top 16, H and I 16384");
+    if (ldx < H || ldy < H) return fail_msg(BM_ERR_SHAPE, "row pitch is smaller than the row length");
+    if (!aligned16(W13) || !aligned16(S13) || !aligned16(W2) || !aligned16(S2) || !aligned_to(workspace, 256))
+        return fail_msg(BM_ERR_ALIGN, "weights and scales must be 16-byte aligned, the workspace 256-byte aligned");
+    if (!aligned_to(X, 2) || !aligned_to(router, 2) || !aligned_to(Y, 2) || !aligned_to(r13, 4) || !aligned_to(r2, 4) || !aligned_to(ids, 4) ||
+        !aligned_to(weights, 4))
+        return fail_msg(BM_ERR_ALIGN, "activations, factors and outputs must be aligned to their elements");
+    const MoeWorkspace w = moe_workspace(T, H, I, E, top);
+    if (workspace_bytes < w.bytes) return fail_msg(BM_ERR_TOO_LARGE, "workspace is smaller than bm_moe_f4_workspace_bytes()");
+    DeviceState* dev = nullptr;
+    if (int rc = current_device_state(&dev)) return rc;
+    // parts of phases that one CTA can get: whole experts in its share, and all passes of the first and the last
+    const int most_passes = ceil_div(T, moe_pass_tokens(ceil_div(H > I ? H : I, 32) * 32));
+    if (T * top / dev->sm_count + 1 + 2 * most_passes > kMoeMaxRuns) return fail_msg(BM_ERR_TOO_LARGE, "too few SMs for this many tokens and experts");
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    MoeParams p{};
+    p.x = static_cast<const uint16_t*>(X);
+    p.router = static_cast<const uint16_t*>(router);
+    p.ldx = ldx;
+    p.ldy = ldy;
+    p.y = static_cast<uint16_t*>(Y);
+    p.ids_out = ids;
+    p.weights_out = weights;
+    p.r13 = r13;
+    p.r2 = r2;
+    p.tokens = T;
+    p.hidden = H;
+    p.inter = I;
+    p.experts = E;
+    p.top = top;
+    p.normalize = normalize != 0;
+    p.x_vec_ok = aligned16(X) && ldx % 8 == 0;
+    p.router_vec_ok = aligned16(router) && H % 8 == 0;
+    p.counters = reinterpret_cast<unsigned*>(ws + w.counters);
+    p.counter_words = w.counter_words;
+    p.x_scale = reinterpret_cast<float*>(ws + w.x_scale);
+    p.ids = reinterpret_cast<int*>(ws + w.ids);
+    p.weights = reinterpret_cast<float*>(ws + w.weights);
+    p.h = reinterpret_cast<float*>(ws + w.h);
+    p.yp = reinterpret_cast<float*>(ws + w.y);
+    p.h_pitch = w.h_pitch;
+    p.y_pitch = w.y_pitch;
+    p.status = dev->status;
+    int clusters = T < 16 ? T : 16;                          // 128 CTAs
+    p.tokens_per_cluster = ceil_div(T, clusters);
+    clusters = ceil_div(T, p.tokens_per_cluster);
+    CUtensorMap mw13, ms13, mw2, ms2;
+    if (int rc = expert_maps(&mw13, &ms13, W13, S13, 2 * E, I, H, format, 2)) return rc;
+    if (int rc = expert_maps(&mw2, &ms2, W2, S2, E, H, I, format, 1)) return rc;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const bool bf16 = x_type == BM_BF16;
+    if (format == BM_F4_E8M0)
+        return bf16 ? launch_moe<FMT_E8M0, true>(mw13, ms13, mw2, ms2, p, clusters, dev->sm_count, st)
+                    : launch_moe<FMT_E8M0, false>(mw13, ms13, mw2, ms2, p, clusters, dev->sm_count, st);
+    return bf16 ? launch_moe<FMT_E4M3, true>(mw13, ms13, mw2, ms2, p, clusters, dev->sm_count, st)
+                : launch_moe<FMT_E4M3, false>(mw13, ms13, mw2, ms2, p, clusters, dev->sm_count, st);
 }
 
 }  // extern "C"

@@ -28,6 +28,7 @@ enum : int {
     DEV_TIMEOUT_DRAIN          = 5,   // teardown waited for copies / MMAs in flight
     DEV_TIMEOUT_SPLITK         = 6,   // split-K consumer waited for partial sums
     DEV_TIMEOUT_PEER           = 7,   // group barrier waited for another GPU's flag
+    DEV_TIMEOUT_EXPERTS        = 8,   // expert layer waited for the other CTAs' part
 };
 
 #ifndef BM_WAIT_LIMIT_NS

@@ -379,6 +379,40 @@ def f4_linear(Xq, Xs, Xr, Wq, Ws, Wr, D, M, N, K, fmt=BM_F4_E4M3):
     return D
 
 
+def moe_f4(X, router, w13, w2, top, inter, fmt=BM_F4_E4M3, normalize=True, out=None, workspace=None):
+    """A mixture-of-experts layer for at most 64 tokens: (Y [T, H], experts int32 [T, top], their weights fp32 [T, top]).
+
+    X [T, H] and router [E, H] fp16 or bf16.  w13, w2: (values, scales, row factors or None) as quantize_f4 gives them with
+    BM_SCALE_ROWS for the experts' matrices one below the other — E * 2 inter rows of H (per expert the gate rows, then
+    the up rows) and E * H rows of inter.  `workspace` (uint8 CUDA tensor) is the call's own until it is done; without one it comes
+    from torch's allocator."""
+    L = _lib.load()
+    if _here(X, "X").dtype not in (torch.float16, torch.bfloat16):
+        raise BmError("X must be float16 or bfloat16")
+    ldx = _f4_rows(X, "X")
+    T, H = X.shape
+    if router.dim() != 2 or router.shape[1] != H:
+        raise BmError(f"router must be a matrix [experts, {H}]")
+    E = router.shape[0]
+    router_ptr = _buffer(router, X.dtype, E * H, "router")
+    a13 = _f4_matrix(*w13, E * 2 * inter, H, fmt, BM_SCALE_ROWS, "w13")
+    a2 = _f4_matrix(*w2, E * H, inter, fmt, BM_SCALE_ROWS, "w2")
+    if out is None:
+        out = torch.empty((T, H), dtype=X.dtype, device=X.device)
+    elif _here(out, "out").dtype != X.dtype or tuple(out.shape) != (T, H):
+        raise BmError(f"out must be a {X.dtype} matrix [{T}, {H}]")
+    ids = torch.empty((T, top), dtype=torch.int32, device=X.device)
+    weights = torch.empty((T, top), dtype=torch.float32, device=X.device)
+    need = L.bm_moe_f4_workspace_bytes(T, H, inter, E, top)
+    if workspace is None:
+        workspace = torch.empty(max(need, 256), dtype=torch.uint8, device=X.device)
+    rc = L.bm_moe_f4(X.data_ptr(), router_ptr, _ELEMENT[X.dtype], *a13, *a2, out.data_ptr(), ids.data_ptr(), weights.data_ptr(),
+                     T, H, inter, E, top, ldx, _f4_rows(out, "out"), fmt, int(bool(normalize)),
+                     _buffer(workspace, torch.uint8, need, "workspace"), workspace.numel(), _stream())
+    _lib.check(rc, "bm_moe_f4")
+    return out, ids, weights
+
+
 def last_device_status() -> int:
     """Status word a bounded in-kernel wait sets when it gives up (0 = none); clears it."""
     import ctypes

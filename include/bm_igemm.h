@@ -286,6 +286,24 @@ int bm_dequantize_f4(const uint8_t *Q, const uint8_t *S, const float *row_scale,
 int bm_f4_gemm(const uint8_t *A, const uint8_t *SA, const float *ra, const uint8_t *W, const uint8_t *SW, const float *rw,
                void *D, int d_type, int M, int N, int K, int64_t ldd, int format, void *stream);
 
+/* A whole mixture-of-experts layer for few tokens, 16-bit activations on 4-bit weights:
+ *   logits = X router^T; every token goes to the `top` experts with the largest logits (of equal ones the lowest index first; a
+ *   NaN counts as smaller than any number), with weights p = softmax over these (normalize != 0) or their share of the softmax
+ *   over all experts;
+ *   Y[t] = sum of p * W2_e (silu(gate) * up), gate and up the two halves of W13_e X[t].
+ * X[T x H] and router[E x H] in `x_type` (BM_F16 or BM_BF16), Y[T x H] in the same type, `ldx` / `ldy` elements between
+ * rows.  W13: E matrices of 2 I rows (I gate rows, then I up rows) and K = H; W2: E matrices of H rows and K = I;
+ * both in `format`, one after the other, scales in BM_SCALE_ROWS; r13 [E * 2 I] and r2 [E * H]: row factors, NULL for ones.
+ * ids and weights [T x top]: the selection, in descending order, may be NULL.  Sums in fp32 (logits in 64 bits); the hidden
+ * activations are rounded once, to 11 bits.  At most 64 tokens, 256 experts, top 16, H and I 16384 (BM_ERR_TOO_LARGE).
+ * `workspace` (>= bm_moe_f4_workspace_bytes, 256-byte aligned, its contents do not matter) belongs to the call until it is
+ * done: calls that may overlap need one each.  Two kernels; the second is a cooperative launch of one CTA per SM. */
+size_t bm_moe_f4_workspace_bytes(int T, int H, int I, int E, int top);
+int bm_moe_f4(const void *X, const void *router, int x_type, const uint8_t *W13, const uint8_t *S13, const float *r13,
+              const uint8_t *W2, const uint8_t *S2, const float *r2, void *Y, int32_t *ids, float *weights, int T, int H,
+              int I, int E, int top, int64_t ldx, int64_t ldy, int format, int normalize, void *workspace,
+              size_t workspace_bytes, void *stream);
+
 /* =======================================================================================
  * Library state
  * ===================================================================================== */

@@ -44,6 +44,28 @@ def test_refusals():
     assert g(D=p + 1) == ALIGN and g(ra=p + 2) == ALIGN and g(t=2, D=p + 2) == ALIGN
 
 
+def test_expert_layer_sizes_and_refusals():
+    L = _lib.load()
+    assert L.bm_moe_f4_workspace_bytes(1, 64, 64, 4, 2) > 0
+    for bad in ((0, 64, 64, 4, 2), (65, 64, 64, 4, 2), (1, 0, 64, 4, 2), (1, 64, 16385, 4, 2), (1, 64, 64, 257, 2), (1, 64, 64, 4, 5), (1, 64, 64, 32, 17)):
+        assert L.bm_moe_f4_workspace_bytes(*bad) == 0
+    buf = np.zeros(4096 + 512, np.uint8)
+    p = (buf.ctypes.data + 255) & ~255
+    names = "x router t w13 s13 r13 w2 s2 r2 y ids wts T H I E top ldx ldy f norm ws wsb st".split()
+    good = dict(x=p, router=p, t=1, w13=p, s13=p, r13=None, w2=p, s2=p, r2=None, y=p, ids=None, wts=None, T=2, H=64, I=32, E=4, top=2, ldx=64, ldy=64,
+                f=1, norm=1, ws=p, wsb=1 << 30, st=None)
+    m = lambda **k: L.bm_moe_f4(*[{**good, **k}[n] for n in names])  # noqa: E731
+    for name in ("x", "router", "w13", "s13", "w2", "s2", "y", "ws"):
+        assert m(**{name: None}) == NULL
+    assert m(f=2) == LAYOUT and m(t=2) == LAYOUT
+    assert m(T=0) == SHAPE and m(H=-1) == SHAPE and m(I=0) == SHAPE and m(E=0) == SHAPE and m(top=0) == SHAPE and m(top=5) == SHAPE
+    assert m(ldx=63) == SHAPE and m(ldy=63) == SHAPE
+    assert m(T=65) == m(H=16385, ldx=20000, ldy=20000) == m(I=16385) == m(E=257) == m(E=32, top=17) == m(wsb=64) == -6
+    for name in ("w13", "s13", "w2", "s2"):
+        assert m(**{name: p + 8}) == ALIGN
+    assert m(ws=p + 128) == ALIGN and m(x=p + 1) == ALIGN and m(y=p + 1) == ALIGN and m(r13=p + 2) == ALIGN and m(ids=p + 1) == ALIGN
+
+
 @pytest.mark.parametrize("fmt", [f4.E8M0, f4.E4M3_FMT])
 def test_the_plain_form_rounds_to_the_nearest(fmt):
     rng = np.random.default_rng(0)
