@@ -164,16 +164,19 @@ static MoeWorkspace moe_workspace(int T, int H, int I, int E, int top) {
     auto up = [](size_t v) { return (v + 255) & ~static_cast<size_t>(255); };
     MoeWorkspace w{};
     const size_t a = static_cast<size_t>(T) * top;
-    w.counter_words = E + 4 + static_cast<int>(a);
-    w.h_pitch = ceil_div(I, 32) * 32;
+    w.counter_words = E + 1;
+    w.split = a <= 16 ? kMoeMaxSplit : a <= 64 ? 2 : 1;      // more assignments than that are units enough
+    w.gu_pitch = 2 * moe_k_blocks(I) * kF4BK;
     w.y_pitch = ceil_div(H, 32) * 32;
     w.counters = 0;
     w.x_scale = w.counters + up(4ull * w.counter_words);
     w.ids = w.x_scale + up(4ull * T);
     w.weights = w.ids + up(4ull * a);
-    w.h = w.weights + up(4ull * a);
-    w.y = w.h + up(4ull * a * w.h_pitch);
-    w.bytes = w.y + up(4ull * a * w.y_pitch);
+    w.x_values = w.weights + up(4ull * a);
+    w.x_scales = w.x_values + up(static_cast<size_t>(T) * moe_value_bytes(H));
+    w.gu = w.x_scales + up(static_cast<size_t>(T) * moe_scale_bytes(H, FMT_E4M3));
+    w.y = w.gu + up(4ull * a * w.split * w.gu_pitch);
+    w.bytes = w.y + up(4ull * a * w.split * w.y_pitch);
     return w;
 }
 static bool moe_in_range(int T, int H, int I, int E, int top) {
@@ -181,13 +184,13 @@ static bool moe_in_range(int T, int H, int I, int E, int top) {
            I > 0 && I <= kMoeMaxDim;
 }
 
-// expert matrices [outer][rows][K]: boxes of 16 rows, as box_outer x (16 / box_outer)
+// expert matrices [outer][rows][K]: boxes of 128 rows, as box_outer x (128 / box_outer)
 static int expert_maps(CUtensorMap* values, CUtensorMap* scales, const uint8_t* q, const uint8_t* s, int outer, int rows, int k, int fmt,
                        uint32_t box_outer) {
     const uint64_t pitch = f4_row_bytes(k), s_pitch = f4_scale_pitch(k, fmt);
     const uint64_t dims[3] = {pitch, static_cast<uint64_t>(rows), static_cast<uint64_t>(outer)};
     const uint64_t s_dims[3] = {s_pitch, static_cast<uint64_t>(rows), static_cast<uint64_t>(outer)};
-    const uint32_t box[3] = {128, 16 / box_outer, box_outer}, s_box[3] = {16, 16 / box_outer, box_outer};
+    const uint32_t box[3] = {128, 128 / box_outer, box_outer}, s_box[3] = {16, 128 / box_outer, box_outer};
     if (int rc = cached_tensor_map(values, q, 3, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, dims, pitch, box, CU_TENSOR_MAP_SWIZZLE_128B, true, pitch * rows))
         return rc;
     return cached_tensor_map(scales, s, 3, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, s_dims, s_pitch, s_box, CU_TENSOR_MAP_SWIZZLE_NONE, true, s_pitch * rows);
@@ -199,7 +202,7 @@ static int launch_moe(const CUtensorMap& w13, const CUtensorMap& s13, const CUte
     auto kern = moe_experts_kernel<FMT, BF16>;
     static ConfiguredFlags flags;
     if (int rc = ensure_smem_limit(flags, kern, kMoeSmemBytes)) return rc;
-    BM_CUDA_TRY(launch_pdl(moe_router_kernel<BF16>, dim3(clusters * kMoeRouterCtas), dim3(kMoeRouterThreads), 0, stream, kMoeRouterCtas, p));
+    BM_CUDA_TRY(launch_pdl(moe_router_kernel<FMT, BF16>, dim3(clusters * kMoeRouterCtas), dim3(kMoeRouterThreads), 0, stream, kMoeRouterCtas, p));
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(ctas);
     cfg.blockDim = dim3(kMoeThreads);
@@ -346,7 +349,7 @@ int bm_moe_f4(const void* X, const void* router, int x_type, const uint8_t* W13,
     DeviceState* dev = nullptr;
     if (int rc = current_device_state(&dev)) return rc;
     // parts of phases that one CTA can get: whole experts in its share, and all passes of the first and the last
-    const int most_passes = ceil_div(T, moe_pass_tokens(ceil_div(H > I ? H : I, 32) * 32));
+    const int most_passes = ceil_div(T, moe_pass_tokens(H > I ? H : I));
     if (T * top / dev->sm_count + 1 + 2 * most_passes > kMoeMaxRuns) return fail_msg(BM_ERR_TOO_LARGE, "too few SMs for this many tokens and experts");
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     MoeParams p{};
@@ -372,9 +375,12 @@ int bm_moe_f4(const void* X, const void* router, int x_type, const uint8_t* W13,
     p.x_scale = reinterpret_cast<float*>(ws + w.x_scale);
     p.ids = reinterpret_cast<int*>(ws + w.ids);
     p.weights = reinterpret_cast<float*>(ws + w.weights);
-    p.h = reinterpret_cast<float*>(ws + w.h);
+    p.x_values = ws + w.x_values;
+    p.x_scales = ws + w.x_scales;
+    p.gu = reinterpret_cast<float*>(ws + w.gu);
     p.yp = reinterpret_cast<float*>(ws + w.y);
-    p.h_pitch = w.h_pitch;
+    p.gu_pitch = w.gu_pitch;
+    p.split = w.split;
     p.y_pitch = w.y_pitch;
     p.status = dev->status;
     int clusters = T < 16 ? T : 16;                          // 128 CTAs

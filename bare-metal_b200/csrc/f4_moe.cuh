@@ -5,24 +5,28 @@
 //
 // What bounds it: every chosen expert's weights are read once, 9/16 (17/32) of a byte a weight; the products are few.
 //
-// Kernel 1, moe_router_kernel: a cluster of 8 CTAs per group of at most 4 tokens.  64 warps share the experts, each
-// token's logits meet in the shared memory of one CTA, whose first warp selects.  Logits are added in fp32 over 8 products and
-// in 64 bits beyond: which expert a token gets must not depend on a sum's rounding or on the batch the token is in.
+// The products run on tcgen05.mma.kind::mxf4nvf4, which takes the weights as they are stored; nothing is done per weight outside
+// the tensor core.  (Converting them to fp16 in registers for mma.sync took 2.2 instructions a weight and reached
+// 1.9 TB/s; the conversion instruction alone runs at 16 weights a clock and SM, a third of what HBM delivers.)  It wants
+// the activations in 4 bits too, so each is a SUM of 6 block-scaled E2M1 numbers: the nearest one, the nearest one to what is
+// left, and so on.  With E4M3 scales what is left shrinks by at least 5.6 a step, with powers of two by 8 after the first: 2^-15 of
+// the block's largest at the end, less than fp16's own rounding of it (2^-12).  The six are six columns of the MMA and cost
+// nothing: an MMA takes as long with 8 columns as with 100.  fp32 sums; a token's six columns are added at the end.
 //
-// Kernel 2, moe_experts_kernel: one CTA per SM, all resident (cooperative launch).  The unit of work is 16 weight rows (gate / up:
-// 8 channels of each) times the tokens of one expert, taken by ONE warp over all of K, so sums never leave registers.  Units are
-// dealt out in contiguous ranges, expert by expert: a CTA keeps its expert's activations in shared memory and
-// meets a new expert once or twice.  A warp streams its rows through a ring of its own (TMA boxes of 16 rows x 256 of K and
-// their scales), refilled by the warp itself as it empties; the refill runs ahead into the next expert and, over
-// the wait for the other CTAs' gate / up results, into the down projection's weights.
-//   The weights become fp16 in registers (cvt e2m1 -> f16, exact) and go through mma.m16n8k16 with fp32 sums: 8 or 16 tokens
-// are the columns, so a weight is converted once for all of them.  tcgen05 would want the activations in 4 or 8 bits too.
-//   E4M3: the scale is multiplied in before the MMA (2 + 4 significant bits, exact in fp16).  E8M0: its range does not fit
-// fp16, so the sums of each block of 32 are scaled in fp32.  Activations are held as fp16 times a power of two per token:
-// fp16 inputs as they are, bf16 inputs moved so that the row's largest is in [2^14, 2^15) (bits below 2^-24 of that, 2^-38 of the
-// largest, are lost), the hidden activations rounded once from fp32 to fp16's 11 bits in the same way.
-//   The experts' outputs go to the workspace in fp32 and are added per token, in the order of the selection, after a last wait:
-// no atomics on sums, the same bits on every call.
+// Kernel 1, moe_router_kernel: a cluster of 8 CTAs per group of at most 4 tokens.  128 warps share the experts, each
+// token's logits meet in the shared memory of one CTA, whose first warp selects, while the other warps cut x into its six parts.
+// Logits are added in fp32 over 8 products and in 64 bits beyond: which expert a token gets must not depend on a sum's
+// rounding or on the batch the token is in.
+//
+// Kernel 2, moe_experts_kernel: one CTA per SM, all resident (cooperative launch).  The unit of work is 128 weight rows (gate / up: 64
+// channels of each) times the tokens of one expert; where units are few they are cut along K, and the parts' sums are
+// added by whoever reads them.  Units are dealt out in contiguous ranges, expert by expert, so a CTA keeps its expert's
+// activations in shared memory.  Weights and scales come through a ring of TMA stages; the scales, stored in rows, are put into
+// tensor memory by four warps (tcgen05.st) on the way.  The ring runs ahead into the next expert and, over the wait
+// for the other CTAs' gate / up sums, into the down projection's weights.
+//   The gate / up sums go to the workspace in fp32; whoever needs an expert's hidden activations waits for its sums, applies
+// SiLU and cuts them into six parts.  The experts' outputs go to the workspace in fp32 and are added per token, in the order of the
+// selection, after a last wait: no atomics on sums, the same bits on every call.
 #pragma once
 #include "f4_format.cuh"
 #include "f4_gemm.cuh"
@@ -34,19 +38,21 @@ constexpr int kMoeMaxTokens = 64;
 constexpr int kMoeMaxExperts = 256;
 constexpr int kMoeMaxTop = 16;
 constexpr int kMoeMaxDim = 16384;
-constexpr int kMoeWarps = 8;
-constexpr int kMoeThreads = 32 * kMoeWarps;
-constexpr int kMoeRing = 5;                                     // ring slots per warp
-constexpr int kMoeItemK = 256;                                  // K of an item: 128 bytes a row
-constexpr int kMoeItemBytes = 16 * 128, kMoeItemScales = 16 * 16;
+constexpr int kMoeParts = 6;                                    // E2M1 numbers an activation is the sum of
+constexpr int kMoeMaxSplit = 4;                                 // pieces of K of a unit at most
 constexpr int kMoeMaxRuns = 112;
-constexpr int kMoeTileTokens = 16;                              // tokens of a pass at most (two MMA column tiles)
-constexpr int kMoeTileBytes = 16 * (8192 + 64);                 // activations of a pass
+
+// Activations cut up: per token and 256 of K 1 KiB, 8 rows (6 used) of 128 bytes in the 128-byte swizzle of an MMA operand, and the
+// scales, per token and tile of 4 blocks 8 rows (6 used) of 4 bytes.
+__host__ __device__ constexpr int moe_k_blocks(int k) { return (k + kF4BK - 1) / kF4BK; }
+__host__ __device__ constexpr int moe_value_bytes(int k) { return moe_k_blocks(k) * 1024; }
+__host__ __device__ constexpr int moe_scale_bytes(int k, int fmt) { return moe_k_blocks(k) * f4_stage_tiles(fmt) * 32; }
 
 struct MoeWorkspace {            // byte offsets
-    size_t counters, x_scale, ids, weights, h, y, bytes;
-    int counter_words;           // done[E], arrived, pad[3], h_max[T * top]
-    int h_pitch, y_pitch;        // elements
+    size_t counters, x_scale, ids, weights, x_values, x_scales, gu, y, bytes;
+    int counter_words;           // done[E], arrived
+    int gu_pitch, y_pitch;       // elements: gate sums and up sums of an assignment (half each); outputs
+    int split;                   // pieces of K that the sums have room for
 };
 
 struct MoeParams {
@@ -67,9 +73,12 @@ struct MoeParams {
     float* x_scale;
     int* ids;
     float* weights;
-    float* h;
+    uint8_t* x_values;
+    uint8_t* x_scales;
+    float* gu;
     float* yp;
-    int h_pitch, y_pitch;
+    int gu_pitch, y_pitch;
+    int split;
     int* status;
 };
 
@@ -97,17 +106,69 @@ __device__ __forceinline__ float dot8(const uint4& a, const uint4& b) {
     return s;
 }
 
-// 2^(14 - floor(log2 m)) and its inverse for a finite m > 0 given as fp32 bits; 1 otherwise (a NaN or infinity shows by itself)
-__device__ __forceinline__ void moe_power(uint32_t bits, float& up, float& down) {
-    const int e = static_cast<int>(bits >> 23);                  // floor(log2 m) + 127
-    up = down = 1.f;
-    if (bits == 0 || e == 255) return;
-    const int n = e < 15 ? 126 : 14 + 127 - e;                   // exponent of `up`, at most 126
-    up = __uint_as_float(static_cast<uint32_t>(n + 127) << 23);
-    down = __uint_as_float(static_cast<uint32_t>(127 - n) << 23);
+// FMT_E4M3: the power of two that puts a row with largest |v| = top (fp32 bits) where the quantiser puts it, and its inverse
+template <int FMT>
+__device__ __forceinline__ void moe_row_factor(uint32_t top_bits, float& factor, float& inv) {
+    factor = inv = 1.f;
+    if (FMT == FMT_E8M0 || top_bits == 0 || top_bits >= 0x7F800000u) return;
+    const int lg = static_cast<int>(top_bits >> 23), e = lg > 11 ? lg - 10 : 1;
+    factor = __uint_as_float(static_cast<uint32_t>(e) << 23);
+    inv = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
 }
 
-constexpr int kMoeRouterCtas = 8, kMoeRouterThreads = 256, kMoeRouterTokens = 4;
+// Eight activations (piece v of a row, two or four neighbouring lanes share a block) cut into E2M1 numbers with scales.  `values`,
+// `scales`: the token's own places, in shared or global memory.  Whole warps; `live` lanes store.
+template <int FMT>
+__device__ __forceinline__ void moe_cut(float (&r)[8], int v, bool live, uint8_t* values, uint8_t* scales) {
+    constexpr int SHARE = f4_block(FMT) / 8;
+    const int block = v / SHARE;
+    uint8_t* row = values + (v >> 5) * 1024 + (v & 3) * 4;
+    uint8_t* scale = scales + (block >> 2) * 32 + (block & 3);
+    const int chunk = (v & 31) >> 2;
+#pragma unroll
+    for (int i = 0; i < kMoeParts; ++i) {
+        uint32_t top = 0;                                         // largest |r|: infinities and NaNs are above all numbers
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(r[j]) & 0x7FFFFFFFu);
+#pragma unroll
+        for (int o = 1; o < SHARE; o <<= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+        const float sixth = __uint_as_float(top) * 0.16666667f;
+        uint32_t byte;
+        float s, inv;
+        if constexpr (FMT == FMT_E4M3) {
+            byte = __nv_cvt_float_to_fp8(sixth, __NV_SATFINITE, __NV_E4M3);
+            s = e4m3_value(byte);
+            inv = s > 0.f ? __fdividef(1.f, s) : 0.f;
+        } else {
+            // the smallest power of two that holds the largest below 6 (or a rounding above it)
+            const uint32_t b = __float_as_uint(sixth);
+            byte = min((b >> 23) + ((b & 0x007FFFFFu) != 0 ? 1u : 0u), 253u);
+            s = e8m0_value(byte);
+            inv = __uint_as_float((254u - byte) << 23);
+        }
+        const bool odd = top >= 0x7F800000u;
+        if (odd) byte = FMT == FMT_E4M3 ? 127u : 255u;
+        float y[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[j] = odd ? 0.f : r[j] * inv;
+        const uint32_t codes = e2m1x8(y);
+        if (live) {
+            *reinterpret_cast<uint32_t*>(row + i * 128 + ((chunk ^ i) << 4)) = codes;
+            if (v % SHARE == 0) scale[i * 4] = static_cast<uint8_t>(byte);
+        }
+        uint32_t h[4];
+        e2m1x8_to_small_half(codes, h);
+        constexpr int kOrder[4] = {1, 3, 0, 2};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float2 f = pair_to_float<false>(h[j]);
+            r[kOrder[j]] = fmaf(f.x * -16384.f, s, r[kOrder[j]]);
+            r[kOrder[j] + 4] = fmaf(f.y * -16384.f, s, r[kOrder[j] + 4]);
+        }
+    }
+}
+
+constexpr int kMoeRouterCtas = 8, kMoeRouterThreads = 512, kMoeRouterTokens = 4;
 
 // order of doubles as unsigned integers, NaN below every number; 0 is left for "no candidate"
 __device__ __forceinline__ unsigned long long logit_key(double v) {
@@ -116,11 +177,12 @@ __device__ __forceinline__ unsigned long long logit_key(double v) {
     return (b < 0 ? ~static_cast<unsigned long long>(b) : static_cast<unsigned long long>(b) | (1ull << 63)) + 2ull;
 }
 
-template <bool BF16>
+template <int FMT, bool BF16>
 __global__ void __launch_bounds__(kMoeRouterThreads)
 moe_router_kernel(const MoeParams p) {
     __shared__ double logits[kMoeMaxExperts];
-    __shared__ uint32_t warp_max[kMoeRouterThreads / 32];
+    constexpr int kWarps = kMoeRouterThreads / 32;
+    __shared__ uint32_t warp_max[kWarps];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = static_cast<int>(cluster_ctarank());
     const int t0 = blockIdx.x / kMoeRouterCtas * p.tokens_per_cluster;
@@ -130,17 +192,47 @@ moe_router_kernel(const MoeParams p) {
     if (blockIdx.x == 0)
         for (int i = threadIdx.x; i < p.counter_words; i += kMoeRouterThreads) p.counters[i] = 0u;
     const int pieces = (p.hidden + 7) / 8;
+    const bool vec_ok = p.x_vec_ok && p.router_vec_ok && p.hidden % 8 == 0;
     cluster_arrive();             // every CTA of the cluster runs: its shared memory may be written
     cluster_wait();
-    for (int e = rank * (kMoeRouterThreads / 32) + warp; e < p.experts; e += kMoeRouterCtas * (kMoeRouterThreads / 32)) {
+    for (int e = rank * kWarps + warp; e < p.experts; e += kMoeRouterCtas * kWarps) {
         const uint16_t* row = p.router + static_cast<size_t>(e) * p.hidden;
         double sum[kMoeRouterTokens] = {0.0, 0.0, 0.0, 0.0};
-#pragma unroll 4
-        for (int v = lane; v < pieces; v += 32) {
-            const uint4 w = moe_piece<BF16>(row, v, p.hidden, p.router_vec_ok);
+        if (vec_ok) {
+            // the loads of several pieces in flight together: beyond the end the last piece again, against zeros
+            constexpr int AHEAD = 8;
+            for (int v0 = lane; v0 < pieces; v0 += 32 * AHEAD) {
+                uint4 w[AHEAD];
 #pragma unroll
-            for (int j = 0; j < kMoeRouterTokens; ++j)
-                if (j < n) sum[j] += static_cast<double>(dot8<BF16>(moe_piece<BF16>(p.x + (t0 + j) * p.ldx, v, p.hidden, p.x_vec_ok), w));
+                for (int i = 0; i < AHEAD; ++i) {
+                    const int v = v0 + 32 * i;
+                    w[i] = __ldg(reinterpret_cast<const uint4*>(row) + min(v, pieces - 1));
+                    if (v >= pieces) w[i] = make_uint4(0, 0, 0, 0);
+                }
+                for (int j = 0; j < n; ++j) {
+                    const uint4* x = reinterpret_cast<const uint4*>(p.x + (t0 + j) * p.ldx);
+                    uint4 d[AHEAD];
+#pragma unroll
+                    for (int i = 0; i < AHEAD; ++i) {
+                        const int v = v0 + 32 * i;
+                        d[i] = __ldg(x + min(v, pieces - 1));
+                        if (v >= pieces) d[i] = make_uint4(0, 0, 0, 0);
+                    }
+                    double s = 0.0;
+#pragma unroll
+                    for (int i = 0; i < AHEAD; ++i) s += static_cast<double>(dot8<BF16>(d[i], w[i]));
+#pragma unroll
+                    for (int k = 0; k < kMoeRouterTokens; ++k)
+                        if (k == j) sum[k] += s;
+                }
+            }
+        } else {
+            for (int v = lane; v < pieces; v += 32) {
+                const uint4 w = moe_piece<BF16>(row, v, p.hidden, p.router_vec_ok);
+#pragma unroll
+                for (int j = 0; j < kMoeRouterTokens; ++j)
+                    if (j < n) sum[j] += static_cast<double>(dot8<BF16>(moe_piece<BF16>(p.x + (t0 + j) * p.ldx, v, p.hidden, p.x_vec_ok), w));
+            }
         }
 #pragma unroll
         for (int j = 0; j < kMoeRouterTokens; ++j) {
@@ -151,12 +243,14 @@ moe_router_kernel(const MoeParams p) {
                 asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(mapa_shared(smem_u32(logits + e), j)), "d"(sum[j]) : "memory");
         }
     }
-    const bool owner = rank < n;                                  // this CTA selects for token t0 + rank
-    if (BF16 && owner) {
-        const uint16_t* row = p.x + (t0 + rank) * p.ldx;
+    // token t0 + rank % 4 is cut up by CTAs rank % 4 and rank % 4 + 4, half of its pieces each
+    const int mine_j = rank & 3, x_pieces = moe_k_blocks(p.hidden) * (kF4BK / 8);
+    const bool cuts = mine_j < n;
+    const uint16_t* x_row = p.x + (t0 + mine_j) * p.ldx;
+    if (FMT == FMT_E4M3 && cuts) {
         uint32_t m = 0;
         for (int v = threadIdx.x; v < pieces; v += kMoeRouterThreads) {
-            const uint4 d = moe_piece<BF16>(row, v, p.hidden, p.x_vec_ok);
+            const uint4 d = moe_piece<BF16>(x_row, v, p.hidden, p.x_vec_ok);
             const uint32_t b = __vmaxu2(__vmaxu2(d.x & 0x7FFF7FFFu, d.y & 0x7FFF7FFFu), __vmaxu2(d.z & 0x7FFF7FFFu, d.w & 0x7FFF7FFFu));
             m = max(m, max(b & 0xFFFFu, b >> 16));
         }
@@ -165,15 +259,36 @@ moe_router_kernel(const MoeParams p) {
     }
     cluster_arrive();
     cluster_wait();
-    if (!owner || warp != 0) return;
-    const int t = t0 + rank;
-    float up = 1.f, down = 1.f;
-    if (BF16) {
-        uint32_t m = lane < kMoeRouterThreads / 32 ? warp_max[lane] : 0u;
-        m = __reduce_max_sync(0xFFFFFFFFu, m);
-        moe_power(m << 16, up, down);
+    if (cuts && warp != 0) {
+        float factor = 1.f, inv = 1.f;
+        if (FMT == FMT_E4M3) {
+            uint32_t m = 0;
+            for (int w = 0; w < kWarps; ++w) m = max(m, warp_max[w]);
+            const float top = BF16 ? __uint_as_float(m << 16) : __half2float(__ushort_as_half(static_cast<unsigned short>(m)));
+            moe_row_factor<FMT>(__float_as_uint(top), factor, inv);
+        }
+        const int t = t0 + mine_j, half = rank >> 2;
+        if (half == 0 && threadIdx.x == 32) p.x_scale[t] = factor;
+        uint8_t* values = p.x_values + static_cast<size_t>(t) * moe_value_bytes(p.hidden);
+        uint8_t* scales = p.x_scales + static_cast<size_t>(t) * moe_scale_bytes(p.hidden, FMT);
+        const int first = half * (x_pieces / 2);
+        for (int v0 = first + (warp - 1) * 32; v0 < first + x_pieces / 2; v0 += (kWarps - 1) * 32) {
+            const int v = v0 + lane;                              // (x_pieces / 2 is a multiple of 16)
+            const bool live = v < first + x_pieces / 2;
+            const uint4 d = live ? moe_piece<BF16>(x_row, v, p.hidden, p.x_vec_ok) : make_uint4(0, 0, 0, 0);
+            const uint32_t w[4] = {d.x, d.y, d.z, d.w};
+            float f[8];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float2 two = pair_to_float<BF16>(w[j]);
+                f[2 * j] = two.x * inv;
+                f[2 * j + 1] = two.y * inv;
+            }
+            moe_cut<FMT>(f, v, live, values, scales);
+        }
     }
-    if (lane == 0) p.x_scale[t] = up;
+    if (rank >= n || warp != 0) return;                           // this CTA's first warp selects for token t0 + rank
+    const int t = t0 + rank;
     constexpr int PER = kMoeMaxExperts / 32;
     unsigned long long key[PER];
 #pragma unroll
@@ -215,166 +330,105 @@ moe_router_kernel(const MoeParams p) {
     }
 }
 
-__device__ __forceinline__ void mma_16x8x16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
-    uint32_t v;
-    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-    return v;
-}
-__device__ __forceinline__ uint4 lds128(uint32_t addr) {
-    uint4 v;
-    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
-    return v;
-}
-__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
-    const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
-    return *reinterpret_cast<const uint32_t*>(&r);
-}
-// scales 2i and 2i + 1 (bytes `sel`) of one word as fp16, each in both halves
-__device__ __forceinline__ void e4m3_pair(uint32_t word, uint32_t sel, uint32_t& s0, uint32_t& s1) {
-    const uint32_t two = __byte_perm(word, 0, sel);
-    uint32_t h;
-    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}\n" : "=r"(h) : "r"(two));
-    s0 = __byte_perm(h, 0, 0x1010);
-    s1 = __byte_perm(h, 0, 0x3232);
-}
+constexpr int kMoeBuilders = 512;                               // warps 2 to 17
+constexpr int kMoeThreads = 64 + kMoeBuilders;                  // TMA producer, MMA issuer, 4 scale warps, 4 epilogue warps, 8 more
+constexpr int kMoeStages = 4;
+constexpr int kMoeTileTokens = 16;                              // tokens of a pass at most: 128 MMA columns
+constexpr int kMoeTileBytes = 128 * 1024;                       // activations of a pass: 8 tokens of 4096, 16 of 2048
+constexpr int kMoeTileScales = 17 * 1024;
+constexpr int kMoeStageValues = 128 * 128, kMoeStageScales = 128 * 16;
+constexpr int kMoeAccStride = 128, kMoeSfBase = 256;            // tensor memory: two accumulators, two sets of scales (32 columns each)
 
-// One item: 16 rows x (32 * chunks) of K against NT tiles of 8 tokens.  Lane (g, q) of a warp (g = lane / 4, q = lane % 4) holds rows
-// g and g + 8 and, of every 32 of K, the 8 from 8 q on; the same 8 of its token's activations: any order of K
-// serves an MMA if both operands keep it.
-template <int FMT, int NT>
-__device__ __forceinline__ void moe_item(uint32_t w, uint32_t scales, uint32_t b_addr, uint32_t b_next, int live, int chunks, int kb, int lane,
-                                         float (&acc)[NT][4]) {
-    const int g = lane >> 2, q = lane & 3;
-    const uint4 sa = lds128(scales + g * 16), sb = lds128(scales + 128 + g * 16);
-    uint32_t s_lo[4], s_hi[4];
-    if constexpr (FMT == FMT_E4M3) {
-        s_lo[0] = sa.x; s_lo[1] = sa.y; s_lo[2] = sa.z; s_lo[3] = sa.w;
-        s_hi[0] = sb.x; s_hi[1] = sb.y; s_hi[2] = sb.z; s_hi[3] = sb.w;
-    } else {                                                      // 16 bytes are 512 of K: this item's half of them
-        s_lo[0] = kb & 1 ? sa.z : sa.x; s_lo[1] = kb & 1 ? sa.w : sa.y;
-        s_hi[0] = kb & 1 ? sb.z : sb.x; s_hi[1] = kb & 1 ? sb.w : sb.y;
-        if (__vcmpeq4(s_lo[0], 0xFFFFFFFFu) | __vcmpeq4(s_lo[1], 0xFFFFFFFFu)) {       // byte 255 is a NaN (the shift below makes it infinity)
-#pragma unroll
-            for (int i = 0; i < NT; ++i) acc[i][0] = acc[i][1] = __uint_as_float(0x7FC00000u);
-        }
-        if (__vcmpeq4(s_hi[0], 0xFFFFFFFFu) | __vcmpeq4(s_hi[1], 0xFFFFFFFFu)) {
-#pragma unroll
-            for (int i = 0; i < NT; ++i) acc[i][2] = acc[i][3] = __uint_as_float(0x7FC00000u);
-        }
-    }
-    const uint32_t row = w + g * 128 + q * 4;
-    const uint32_t sel = q < 2 ? 0x4420u : 0x4431u;               // blocks of 16: lanes 0, 1 the first, lanes 2, 3 the second of a chunk
-    uint32_t m0[2], m1[2];
-#pragma unroll
-    for (int c = 0; c < 8; ++c) {
-        if (c >= chunks) break;
-        uint32_t h0[4], h1[4];
-        const uint32_t at = row + ((c ^ g) << 4);                 // 128-byte swizzle
-        e2m1x8_to_half(lds32(at), h0);
-        e2m1x8_to_half(lds32(at + 1024), h1);
-        if constexpr (FMT == FMT_E4M3) {
-            if ((c & 1) == 0) {
-                e4m3_pair(s_lo[c >> 1], sel, m0[0], m0[1]);
-                e4m3_pair(s_hi[c >> 1], sel, m1[0], m1[1]);
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                h0[j] = hmul2(h0[j], m0[c & 1]);
-                h1[j] = hmul2(h1[j], m1[c & 1]);
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < NT; ++i) {
-            uint4 b = make_uint4(0, 0, 0, 0);
-            if (g + 8 * i < live) b = lds128(b_addr + i * b_next + c * 64);
-            if constexpr (FMT == FMT_E4M3) {
-                mma_16x8x16(acc[i], h0[0], h1[0], h0[1], h1[1], b.x, b.y);
-                mma_16x8x16(acc[i], h0[2], h1[2], h0[3], h1[3], b.z, b.w);
-            } else {
-                float part[4] = {0.f, 0.f, 0.f, 0.f};
-                mma_16x8x16(part, h0[0], h1[0], h0[1], h1[1], b.x, b.y);
-                mma_16x8x16(part, h0[2], h1[2], h0[3], h1[3], b.z, b.w);
-                // byte c of the row's scales << 23 (byte 0 stands for 2^-127, here for 0: nothing in fp32)
-                const float f0 = __uint_as_float(__byte_perm(s_lo[c >> 2], 0, 0x0444 | ((c & 3) << 12)) >> 1);
-                const float f1 = __uint_as_float(__byte_perm(s_hi[c >> 2], 0, 0x0444 | ((c & 3) << 12)) >> 1);
-                acc[i][0] = fmaf(part[0], f0, acc[i][0]);
-                acc[i][1] = fmaf(part[1], f0, acc[i][1]);
-                acc[i][2] = fmaf(part[2], f1, acc[i][2]);
-                acc[i][3] = fmaf(part[3], f1, acc[i][3]);
-            }
-        }
-    }
+__host__ __device__ constexpr int moe_pass_tokens(int k) {       // an even number
+    const int n = kMoeTileBytes / moe_value_bytes(k);
+    return n < kMoeTileTokens ? n / 2 * 2 : kMoeTileTokens;
 }
+__host__ __device__ constexpr int moe_tile_scale_pitch(int k, int fmt) { return moe_scale_bytes(k, fmt) + 32; }   // tokens 8 banks apart
 
-// Part of a phase's work that one CTA does with one tile of activations: units [first, last) of an expert, tokens of one pass.
+// Part of a phase's work that one CTA does with one tile of activations: elements [first, last) of an expert (element = unit *
+// pieces of K + piece), tokens of one pass.
 struct MoeRun {
     uint16_t expert, pass, first, last;
 };
 
 struct MoeShared {
     unsigned long long token_mask[kMoeMaxExperts];
-    int start[2][kMoeMaxExperts + 1];            // work before each expert, per phase
+    int start[2][kMoeMaxExperts + 1];            // units x passes before each expert, per phase
     MoeRun runs[2][kMoeMaxRuns];
-    int run_count[2];
-    int slot_row[kMoeTileTokens];                // assignment (token * top + choice) of each token of the pass
-    float slot_scale[kMoeTileTokens];            // what a sum of the pass is multiplied with
+    int run_count[2], split[2];
+    int slot_row[4][kMoeTileTokens];             // per run (mod 4): assignment (token * top + choice) of each token of the pass
+    float slot_scale[4][kMoeTileTokens];         // what its sums are multiplied with
+    uint32_t slot_top[kMoeTileTokens];           // largest hidden activation, fp32 bits
     int abort_flag;
-    unsigned long long full[kMoeWarps * kMoeRing];
+    uint32_t tmem_slot;
+    unsigned long long full[kMoeStages], empty[kMoeStages], sf_full[2], sf_empty[2], acc_full[2], acc_empty[2], tile_full[2], tile_empty, drain;
 };
-constexpr int kMoeRingOffset = 0;
-constexpr int kMoeScaleOffset = kMoeWarps * kMoeRing * kMoeItemBytes;
-constexpr int kMoeTileOffset = kMoeScaleOffset + kMoeWarps * kMoeRing * kMoeItemScales;
-constexpr int kMoeSharedOffset = kMoeTileOffset + kMoeTileBytes;
+constexpr int kMoeStageScaleOffset = kMoeStages * kMoeStageValues;
+constexpr int kMoeTileOffset = kMoeStageScaleOffset + kMoeStages * kMoeStageScales;
+constexpr int kMoeTileScaleOffset = kMoeTileOffset + kMoeTileBytes;
+constexpr int kMoeSharedOffset = kMoeTileScaleOffset + kMoeTileScales;
 constexpr int kMoeSmemBytes = kMoeSharedOffset + static_cast<int>(sizeof(MoeShared)) + 1024;
 static_assert(kMoeSmemBytes <= 227 * 1024, "shared memory over-subscribed");
 
-__host__ __device__ constexpr int moe_tile_pitch(int k_padded) { return (2 * k_padded + 63) / 128 * 128 + 64; }   // 64 mod 128: no bank conflicts
-__host__ __device__ constexpr int moe_pass_tokens(int k_padded) {
-    const int n = kMoeTileBytes / moe_tile_pitch(k_padded);
-    return n < kMoeTileTokens ? n : kMoeTileTokens;
+__device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};"
+        ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+          "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
+        : "memory");
 }
-
-// A warp's own sequence of items: phase, run, unit, K.
-struct MoeCursor {
-    int phase, run, unit, kb;
-    bool done;
-};
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void builders_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kMoeBuilders) : "memory"); }
 
 template <int FMT, bool BF16>
 __global__ void __launch_bounds__(kMoeThreads, 1)
 moe_experts_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_constant__ CUtensorMap map_s13,
                    const __grid_constant__ CUtensorMap map_w2, const __grid_constant__ CUtensorMap map_s2, const MoeParams p) {
+    constexpr int KT = f4_stage_tiles(FMT);
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
     MoeShared& sh = *reinterpret_cast<MoeShared*>(smem_gen + kMoeSharedOffset);
     uint8_t* tile = smem_gen + kMoeTileOffset;
+    uint8_t* tile_scales = smem_gen + kMoeTileScaleOffset;
     const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-    const int g = lane >> 2, q = lane & 3;
-    const uint32_t ring = smem_base + warp * kMoeRing * kMoeItemBytes, ring_scales = smem_base + kMoeScaleOffset + warp * kMoeRing * kMoeItemScales;
-    const uint32_t full0 = smem_u32(sh.full + warp * kMoeRing);
     volatile int* abort_flag = &sh.abort_flag;
     unsigned* done = p.counters;
     unsigned* arrived = p.counters + p.experts;
-    unsigned* h_max = p.counters + p.experts + 4;
+    auto bar_of = [&](const unsigned long long& b) { return smem_u32(&b); };
 
-    const int k_padded[2] = {(p.hidden + 31) / 32 * 32, (p.inter + 31) / 32 * 32};
-    const int units[2] = {(p.inter + 7) / 8, (p.hidden + 15) / 16};
-    const int pass_tokens[2] = {moe_pass_tokens(k_padded[0]), moe_pass_tokens(k_padded[1])};
+    const int units[2] = {(p.inter + 63) / 64, (p.hidden + 127) / 128};
+    const int pass_tokens[2] = {moe_pass_tokens(p.hidden), moe_pass_tokens(p.inter)};
+    const int items[2] = {moe_k_blocks(p.hidden), moe_k_blocks(p.inter)};
 
     // ---- who does what: token sets of the experts, work before each expert, this CTA's runs
     for (int e = threadIdx.x; e < p.experts; e += kMoeThreads) sh.token_mask[e] = 0ull;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < kMoeWarps * kMoeRing; ++i) mbar_init(smem_u32(sh.full + i), 1);
+        for (int i = 0; i < kMoeStages; ++i) {
+            mbar_init(bar_of(sh.full[i]), 1);
+            mbar_init(bar_of(sh.empty[i]), 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(bar_of(sh.sf_full[i]), 4);
+            mbar_init(bar_of(sh.sf_empty[i]), 1);
+            mbar_init(bar_of(sh.acc_full[i]), 1);
+            mbar_init(bar_of(sh.acc_empty[i]), 4);
+        }
+        mbar_init(bar_of(sh.tile_full[0]), 1);                   // gate / up: copies of what the router kernel cut
+        mbar_init(bar_of(sh.tile_full[1]), kMoeBuilders / 32);   // down: cut here
+        mbar_init(bar_of(sh.tile_empty), 1);
+        mbar_init(bar_of(sh.drain), 1);
         sh.abort_flag = 0;
         fence_mbar_init();
     }
+    if (warp == 1) {
+        tmem_alloc(smem_u32(&sh.tmem_slot), 512);
+        tmem_relinquish();
+    }
+    tc_fence_before_sync();
     __syncthreads();
+    tc_fence_after_sync();
+    const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(&sh.tmem_slot);
     for (int a = threadIdx.x; a < p.tokens * p.top; a += kMoeThreads) atomicOr(&sh.token_mask[p.ids[a]], 1ull << (a / p.top));
     __syncthreads();
     if (warp < 2) {
@@ -392,222 +446,348 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_con
             if (e < p.experts) sh.start[ph][e] = carry + sum - mine;
             carry += __shfl_sync(0xFFFFFFFFu, sum, 31);
         }
-        if (lane == 0) sh.start[ph][p.experts] = carry;
+        // pieces of K: as few as leave no CTA with much more than its share (one piece more costs about a twentieth of a unit)
+        int split = 1;
+        float best = 1e30f;
+        for (int s = 1; s <= min(p.split, items[ph]); ++s) {
+            const float cost = static_cast<float>((carry * s + gridDim.x - 1) / gridDim.x) / s + 0.05f * s;
+            if (cost < best) { best = cost; split = s; }
+        }
+        if (lane == 0) {
+            sh.start[ph][p.experts] = carry;
+            sh.split[ph] = split;
+        }
         __syncwarp();
-        const long long total = carry;
+        const long long total = static_cast<long long>(carry) * split;
         const int from = static_cast<int>(total * blockIdx.x / gridDim.x), to = static_cast<int>(total * (blockIdx.x + 1) / gridDim.x);
         int count = 0;
         for (int e0 = 0; e0 < p.experts; e0 += 32) {
             const int e = e0 + lane;
-            const bool hit = e < p.experts && sh.start[ph][e] < to && sh.start[ph][e + 1] > from && sh.start[ph][e] < sh.start[ph][e + 1];
-            unsigned todo = __ballot_sync(0xFFFFFFFFu, hit);
+            const int lo = e < p.experts ? sh.start[ph][e] * split : 0, hi = e < p.experts ? sh.start[ph][e + 1] * split : 0;
+            unsigned todo = __ballot_sync(0xFFFFFFFFu, lo < hi && lo < to && hi > from);
             while (todo) {
                 const int ex = e0 + __ffs(todo) - 1;
                 todo &= todo - 1;
-                const int base = sh.start[ph][ex], passes = (sh.start[ph][ex + 1] - base) / units[ph];
-                const int a = max(from, base) - base, b = min(to, sh.start[ph][ex + 1]) - base;
-                // position = unit * passes + pass: the passes over the same rows follow one another
-                for (int pass = lane; pass < passes; pass += 32) {
+                const int base = sh.start[ph][ex] * split, end = sh.start[ph][ex + 1] * split;
+                const int passes = (end - base) / (units[ph] * split);
+                const int a = max(from, base) - base, b = min(to, end) - base;
+                // position = element * passes + pass: the passes over the same rows follow one another
+                for (int p0 = 0; p0 < passes; p0 += 32) {
+                    const int pass = p0 + lane;
                     const int first = a > pass ? (a - pass + passes - 1) / passes : 0, last = b > pass ? (b - pass + passes - 1) / passes : 0;
-                    if (count + pass < kMoeMaxRuns)
-                        sh.runs[ph][count + pass] = MoeRun{static_cast<uint16_t>(ex), static_cast<uint16_t>(pass), static_cast<uint16_t>(first),
-                                                           static_cast<uint16_t>(last)};
+                    const unsigned some = __ballot_sync(0xFFFFFFFFu, pass < passes && first < last);
+                    const int at = count + __popc(some & ((1u << lane) - 1u));
+                    if (((some >> lane) & 1u) && at < kMoeMaxRuns)
+                        sh.runs[ph][at] = MoeRun{static_cast<uint16_t>(ex), static_cast<uint16_t>(pass), static_cast<uint16_t>(first),
+                                                 static_cast<uint16_t>(last)};
+                    count += __popc(some);
                 }
-                count += passes;
             }
         }
         if (lane == 0) sh.run_count[ph] = count < kMoeMaxRuns ? count : kMoeMaxRuns;
     }
     __syncthreads();
-
-    // ---- a warp's items and its ring
-    auto settle = [&](MoeCursor& c) {                             // on to the next unit of this warp, if (c.unit) is past its run
-        for (;;) {
-            if (c.run >= sh.run_count[c.phase]) {
-                if (c.phase == 1) { c.done = true; return; }
-                c.phase = 1;
-                c.run = 0;
-                if (sh.run_count[1] > 0) c.unit = sh.runs[1][0].first + warp;
-                continue;
-            }
-            if (c.unit < sh.runs[c.phase][c.run].last) return;
-            if (++c.run < sh.run_count[c.phase]) c.unit = sh.runs[c.phase][c.run].first + warp;
-        }
+    const int count0 = sh.run_count[0], runs = count0 + sh.run_count[1];
+    auto run_tokens = [&](const MoeRun& r, int ph) { return min(pass_tokens[ph], __popcll(sh.token_mask[r.expert]) - r.pass * pass_tokens[ph]); };
+    // the assignment that token number j of a run's pass is
+    auto slot_of = [&](const MoeRun& r, int ph, int j) {
+        unsigned long long m = sh.token_mask[r.expert];
+        for (int i = 0; i < r.pass * pass_tokens[ph] + j; ++i) m &= m - 1;
+        const int t = __ffsll(static_cast<long long>(m)) - 1;
+        int choice = 0;
+        while (choice < p.top - 1 && p.ids[t * p.top + choice] != r.expert) ++choice;
+        return t * p.top + choice;
     };
-    MoeCursor ahead{0, 0, sh.run_count[0] > 0 ? sh.runs[0][0].first + warp : 0, 0, false};
-    settle(ahead);
-    uint32_t issued = 0, taken = 0;
-    auto refill = [&] {                                           // the next item into the slot that `issued` names
-        if (ahead.done) return;
-        const int slot = issued % kMoeRing;
-        const uint32_t bar = full0 + 8u * slot;
-        const int expert = sh.runs[ahead.phase][ahead.run].expert;
-        if (elect_one()) {
-            mbar_expect_tx(bar, kMoeItemBytes + kMoeItemScales);
-            const int sx = (FMT == FMT_E4M3 ? ahead.kb : ahead.kb >> 1) * 16;
-            if (ahead.phase == 0) {
-                tma_load_3d(ring + slot * kMoeItemBytes, &map_w13, bar, ahead.kb * 128, ahead.unit * 8, expert * 2);
-                tma_load_3d(ring_scales + slot * kMoeItemScales, &map_s13, bar, sx, ahead.unit * 8, expert * 2);
-            } else {
-                tma_load_3d(ring + slot * kMoeItemBytes, &map_w2, bar, ahead.kb * 128, ahead.unit * 16, expert);
-                tma_load_3d(ring_scales + slot * kMoeItemScales, &map_s2, bar, sx, ahead.unit * 16, expert);
+
+    // Every role goes through the CTA's runs, their elements and these elements' stages in the same order.
+    if (warp == 0) {
+        // ------------------------------------------------------------------ producer: weights and their scales
+        uint32_t stage = 0, phase = 0;
+        bool ok = true;
+        for (int it = 0; it < runs && ok; ++it) {
+            const int ph = it >= count0, split = sh.split[ph];
+            const MoeRun r = sh.runs[ph][ph ? it - count0 : it];
+            const CUtensorMap* values = ph ? &map_w2 : &map_w13;
+            const CUtensorMap* scales = ph ? &map_s2 : &map_s13;
+            for (int el = r.first; el < r.last && ok; ++el) {
+                const int unit = el / split, piece = el - unit * split;
+                const int kb1 = items[ph] * (piece + 1) / split, row = unit * (ph ? 128 : 64), outer = ph ? r.expert : 2 * r.expert;
+                for (int kb = items[ph] * piece / split; kb < kb1; ++kb) {
+                    if (!warp_bounded_wait(bar_of(sh.empty[stage]), phase ^ 1u, abort_flag, p.status, DEV_TIMEOUT_PRODUCER_EMPTY)) { ok = false; break; }
+                    if (elect_one()) {
+                        const uint32_t bar = bar_of(sh.full[stage]);
+                        mbar_expect_tx(bar, kMoeStageValues + kMoeStageScales);
+                        tma_load_3d(smem_base + stage * kMoeStageValues, values, bar, kb * 128, row, outer);
+                        tma_load_3d(smem_base + kMoeStageScaleOffset + stage * kMoeStageScales, scales, bar, (FMT == FMT_E4M3 ? kb : kb >> 1) * 16, row, outer);
+                    }
+                    __syncwarp();
+                    if (++stage == kMoeStages) { stage = 0; phase ^= 1u; }
+                }
             }
         }
-        __syncwarp();
-        ++issued;
-        if (++ahead.kb * kMoeItemK >= k_padded[ahead.phase]) {
-            ahead.kb = 0;
-            ahead.unit += kMoeWarps;
-            settle(ahead);
-        }
-    };
-    for (int i = 0; i < kMoeRing; ++i) refill();
-
-    bool ok = true;
-    for (int ph = 0; ph < 2 && ok; ++ph) {
-        const int kp = k_padded[ph], pitch = moe_tile_pitch(kp), items = (kp + kMoeItemK - 1) / kMoeItemK;
-        for (int run = 0; run < sh.run_count[ph] && ok; ++run) {
+    } else if (warp == 1) {
+        // ------------------------------------------------------------------ MMA issuer
+        uint32_t stage = 0, phase = 0, buf = 0, buf_phase = 0, acc = 0, acc_phase = 0;
+        bool ok = true;
+        for (int it = 0; it < runs && ok; ++it) {
+            const int ph = it >= count0, run = ph ? it - count0 : it, split = sh.split[ph];
             const MoeRun r = sh.runs[ph][run];
-            const unsigned long long mask = sh.token_mask[r.expert];
-            const int of_expert = __popcll(mask);
-            const int n = r.first < r.last ? min(pass_tokens[ph], of_expert - r.pass * pass_tokens[ph]) : 0;   // (a run may be empty)
-            __syncthreads();                                      // the tile before has been read, the run before is complete
-            if (ph == 0 && run > 0 && threadIdx.x == 0) {
-                const MoeRun b = sh.runs[0][run - 1];
-                __threadfence();
-                atomicAdd(done + b.expert, static_cast<unsigned>(b.last - b.first));
-            }
-            if (static_cast<int>(threadIdx.x) < n) {
-                unsigned long long m = mask;
-                for (int i = 0; i < r.pass * pass_tokens[ph] + static_cast<int>(threadIdx.x); ++i) m &= m - 1;
-                const int t = __ffsll(static_cast<long long>(m)) - 1;
-                int choice = 0;
-                while (choice < p.top - 1 && p.ids[t * p.top + choice] != r.expert) ++choice;
-                sh.slot_row[threadIdx.x] = t * p.top + choice;
-            }
-            if (ph == 1 && n > 0 && threadIdx.x == 0) {
-                // the expert's hidden activations come from several CTAs
-                const unsigned want = static_cast<unsigned>(sh.start[0][r.expert + 1] - sh.start[0][r.expert]);
-                const uint64_t t0 = global_timer_ns();
-                for (;;) {
-                    unsigned v;
-                    asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(done + r.expert) : "memory");
-                    if (v >= want) break;
-                    if (global_timer_ns() - t0 > BM_WAIT_LIMIT_NS) {
-                        *abort_flag = 1;
-                        if (p.status) atomicCAS(p.status, 0, DEV_TIMEOUT_EXPERTS);
-                        break;
-                    }
-                }
-            }
-            __syncthreads();
-            if (*abort_flag) { ok = false; break; }
-            // ---- activations of the pass: fp16 rows, zeros up to whole 32s
-            for (int j = 0; j < n; ++j) {
-                const int row = sh.slot_row[j];
-                uint4* dst = reinterpret_cast<uint4*>(tile + j * pitch);
-                if (ph == 0) {
-                    const int t = row / p.top;
-                    const float up = BF16 ? __ldcg(p.x_scale + t) : 1.f;
-                    if (threadIdx.x == 0) sh.slot_scale[j] = __frcp_rn(up);                 // a power of two
-                    const uint16_t* src = p.x + t * p.ldx;
-                    for (int v = threadIdx.x; v < kp / 8; v += kMoeThreads) {
-                        uint4 d = moe_piece<BF16>(src, v, p.hidden, p.x_vec_ok);
-                        if constexpr (BF16) {
-                            uint32_t* w = reinterpret_cast<uint32_t*>(&d);
+            const int columns = (run_tokens(r, ph) + 1) / 2 * 16;
+            const uint32_t idesc0 = make_idesc_f4<FMT>(128, columns, 0), idesc2 = make_idesc_f4<FMT>(128, columns, 2);
+            if (!warp_bounded_wait(bar_of(sh.tile_full[ph]), run & 1, abort_flag, p.status, DEV_TIMEOUT_MMA_FULL)) { ok = false; break; }
+            for (int el = r.first; el < r.last && ok; ++el) {
+                const int unit = el / split, piece = el - unit * split;
+                const int kb0 = items[ph] * piece / split, kb1 = items[ph] * (piece + 1) / split;
+                if (!warp_bounded_wait(bar_of(sh.acc_empty[acc]), acc_phase ^ 1u, abort_flag, p.status, DEV_TIMEOUT_MMA_ACC_EMPTY)) { ok = false; break; }
+                for (int kb = kb0; kb < kb1; ++kb) {
+                    if (!warp_bounded_wait(bar_of(sh.full[stage]), phase, abort_flag, p.status, DEV_TIMEOUT_MMA_FULL) ||
+                        !warp_bounded_wait(bar_of(sh.sf_full[buf]), buf_phase, abort_flag, p.status, DEV_TIMEOUT_MMA_FULL)) { ok = false; break; }
+                    tc_fence_after_sync();
+                    if (elect_one()) {
+                        const uint32_t d = tmem_base + acc * kMoeAccStride, sfa = tmem_base + kMoeSfBase + buf * 32, sfb = sfa + 16;
+                        const uint64_t a_desc = make_smem_desc(smem_base + stage * kMoeStageValues, 0, 1024, SWIZZLE_128B_DESC);
+                        // the 8 columns of a token are one row group; the groups lie a token's activations apart
+                        const uint64_t b_desc = make_smem_desc(smem_base + kMoeTileOffset + kb * 1024, 0, items[ph] * 1024, SWIZZLE_128B_DESC);
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const float2 f = pair_to_float<true>(w[i]);
-                                w[i] = float_to_pair<false>(__fmul_rn(f.x, up), __fmul_rn(f.y, up));
-                            }
+                        for (int ks = 0; ks < 4; ++ks) {
+                            const int t = ks * KT / 4;
+                            mma_f4<false, FMT>(d, a_desc + ks * 2, b_desc + ks * 2, FMT == FMT_E8M0 && (ks & 1) ? idesc2 : idesc0, sfa + t * 4, sfb + t * 4,
+                                               (kb != kb0 || ks != 0) ? 1u : 0u);
                         }
-                        dst[v] = d;
+                        tc_commit(bar_of(sh.empty[stage]));
+                        tc_commit(bar_of(sh.sf_empty[buf]));
                     }
-                } else {
-                    float up, down;
-                    moe_power(__ldcg(h_max + row), up, down);
-                    if (threadIdx.x == 0) sh.slot_scale[j] = down;
-                    const float* src = p.h + static_cast<size_t>(row) * p.h_pitch;
-                    for (int v = threadIdx.x; v < kp / 8; v += kMoeThreads) {
-                        const float4 lo = __ldcg(reinterpret_cast<const float4*>(src) + 2 * v), hi = __ldcg(reinterpret_cast<const float4*>(src) + 2 * v + 1);
-                        float f[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) f[i] = v * 8 + i < p.inter ? __fmul_rn(f[i], up) : 0.f;     // nobody wrote what is behind
-                        dst[v] = make_uint4(float_to_pair<false>(f[0], f[1]), float_to_pair<false>(f[2], f[3]), float_to_pair<false>(f[4], f[5]),
-                                            float_to_pair<false>(f[6], f[7]));
-                    }
-                }
-            }
-            __syncthreads();
-            const uint32_t b_lane = smem_u32(tile) + g * pitch + q * 16, b_next = 8u * pitch;
-            for (int unit = r.first + warp; unit < r.last && ok; unit += kMoeWarps) {
-                float acc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-                for (int kb = 0; kb < items; ++kb) {
-                    const int slot = taken % kMoeRing;
-                    if (!warp_bounded_wait(full0 + 8u * slot, (taken / kMoeRing) & 1u, abort_flag, p.status, DEV_TIMEOUT_MMA_FULL)) { ok = false; break; }
-                    ++taken;
-                    const int left = kp / 32 - kb * 8, chunks = left < 8 ? left : 8;
-                    const uint32_t w = ring + slot * kMoeItemBytes, s = ring_scales + slot * kMoeItemScales;
-                    if (n <= 8) moe_item<FMT, 1>(w, s, b_lane + kb * 512, b_next, n, chunks, kb, lane, reinterpret_cast<float(&)[1][4]>(acc));
-                    else moe_item<FMT, 2>(w, s, b_lane + kb * 512, b_next, n, chunks, kb, lane, acc);
-                    __syncwarp();                                 // all lanes have read the slot
-                    refill();
+                    __syncwarp();
+                    if (++stage == kMoeStages) { stage = 0; phase ^= 1u; }
+                    buf ^= 1u;
+                    if (buf == 0) buf_phase ^= 1u;
                 }
                 if (!ok) break;
-                if (ph == 0) {
-                    // rows g: gate, rows g + 8: up of channel unit * 8 + g
-                    const int channel = unit * 8 + g;
-                    const bool in = channel < p.inter;
-                    const size_t base = static_cast<size_t>(r.expert) * 2 * p.inter;
-                    const float fg = in && p.r13 ? __ldg(p.r13 + base + channel) : 1.f;
-                    const float fu = in && p.r13 ? __ldg(p.r13 + base + p.inter + channel) : 1.f;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int j = (i >> 1) * 8 + q * 2 + (i & 1);
-                        if ((i >> 1) * 8 >= n) break;
-                        float hv = 0.f;
-                        if (j < n) {
-                            const float s = sh.slot_scale[j];
-                            const float gate = acc[i >> 1][i & 1] * fg * s, up = acc[i >> 1][2 + (i & 1)] * fu * s;
-                            hv = gate / (1.f + expf(-gate)) * up;
-                            if (in) __stcg(p.h + static_cast<size_t>(sh.slot_row[j]) * p.h_pitch + channel, hv);
-                            else hv = 0.f;
+                if (elect_one()) tc_commit(bar_of(sh.acc_full[acc]));
+                __syncwarp();
+                acc ^= 1u;
+                if (acc == 0) acc_phase ^= 1u;
+            }
+            if (!ok) break;
+            if (elect_one()) tc_commit(bar_of(sh.tile_empty));
+            __syncwarp();
+        }
+        if (!ok) {
+            if (elect_one()) tc_commit(bar_of(sh.drain));
+            __syncwarp();
+            const uint64_t t0 = global_timer_ns();
+            while (!mbar_try_wait(bar_of(sh.drain), 0) && global_timer_ns() - t0 < 20000000ull) {}
+        }
+    } else {
+        // ------------------------------------------------------------------ builders; among them scale warps and epilogue warps
+        const int quarter = warp & 3, tid = static_cast<int>(threadIdx.x) - 64;
+        const bool scales_role = warp < 6, epilogue_role = warp >= 6 && warp < 10;
+        uint32_t stage = 0, phase = 0, buf = 0, buf_phase = 0, acc = 0, acc_phase = 0;
+        bool ok = true;                                           // a warp that gave up still meets the others at their barriers
+        for (int it = 0; it < runs; ++it) {
+            const int ph = it >= count0, run = ph ? it - count0 : it, split = sh.split[ph], k = ph ? p.inter : p.hidden;
+            const MoeRun r = sh.runs[ph][run];
+            const int n = run_tokens(r, ph), value_bytes = moe_value_bytes(k), scale_pitch = moe_tile_scale_pitch(k, FMT);
+            int* slot_row = sh.slot_row[it & 3];
+            float* slot_scale = sh.slot_scale[it & 3];
+            // the tile of the run before has been read.  The scale and epilogue warps know by their own work up to the last run but one
+            // that it is this phase of the barrier that they look at; the others keep up with every run.
+            if (ph == 1 || (!scales_role && !epilogue_role))
+                ok = ok && (it == 0 || warp_bounded_wait(bar_of(sh.tile_empty), (it - 1) & 1, abort_flag, p.status, DEV_TIMEOUT_PRODUCER_EMPTY));
+            if (ph == 0) {
+                if (warp == 10) {                                 // copies what the router kernel has cut
+                    if (ok) {
+                        const uint32_t bar = bar_of(sh.tile_full[0]);
+                        const int scale_bytes = moe_scale_bytes(k, FMT);
+                        int t = 0;
+                        if (lane < n) {
+                            const int row = slot_of(r, 0, lane);
+                            t = row / p.top;
+                            slot_row[lane] = row;
+                            slot_scale[lane] = p.x_scale[t];
                         }
-                        uint32_t m = __float_as_uint(fabsf(hv));
-#pragma unroll
-                        for (int o = 4; o < 32; o <<= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-                        if (g == 0 && j < n && m != 0u) atomicMax(h_max + sh.slot_row[j], m);
-                    }
-                } else {
-#pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        const int channel = unit * 16 + half * 8 + g;
-                        if (channel >= p.hidden) continue;
-                        const float f = p.r2 ? __ldg(p.r2 + static_cast<size_t>(r.expert) * p.hidden + channel) : 1.f;
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const int j = (i >> 1) * 8 + q * 2 + (i & 1);
-                            if (j < n) __stcg(p.yp + static_cast<size_t>(sh.slot_row[j]) * p.y_pitch + channel,
-                                              acc[i >> 1][half * 2 + (i & 1)] * f * sh.slot_scale[j]);
+                        __syncwarp();
+                        if (lane == 0) mbar_expect_tx(bar, n * (value_bytes + scale_bytes));
+                        __syncwarp();
+                        if (lane < n) {
+                            bulk_load(smem_u32(tile) + lane * value_bytes, p.x_values + static_cast<size_t>(t) * value_bytes, value_bytes, bar);
+                            bulk_load(smem_u32(tile_scales) + lane * scale_pitch, p.x_scales + static_cast<size_t>(t) * scale_bytes, scale_bytes, bar);
                         }
                     }
                 }
+            } else {
+                // ---- hidden activations of the pass: silu(gate) * up from the sums of all CTAs, cut into their parts
+                if (tid < n) {
+                    slot_row[tid] = slot_of(r, 1, tid);
+                    sh.slot_top[tid] = 0u;
+                }
+                if (tid == 32) {
+                    const unsigned want = static_cast<unsigned>(sh.start[0][r.expert + 1] - sh.start[0][r.expert]) * sh.split[0] * 4u;
+                    const uint64_t t0 = global_timer_ns();
+                    while (!*abort_flag) {
+                        unsigned v;
+                        asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(done + r.expert) : "memory");
+                        if (v >= want) break;
+                        if (global_timer_ns() - t0 > BM_WAIT_LIMIT_NS) {
+                            *abort_flag = 1;
+                            if (p.status) atomicCAS(p.status, 0, DEV_TIMEOUT_EXPERTS);
+                        }
+                    }
+                }
+                builders_sync();
+                const int row_pieces = items[1] * (kF4BK / 8);    // a multiple of 32: a warp's pieces are one token's
+                const int split0 = sh.split[0];
+                auto hidden = [&](int j, int v, float (&h)[8]) {
+                    const float* src = p.gu + static_cast<size_t>(slot_row[j]) * p.split * p.gu_pitch + v * 8;
+                    float up[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) h[i] = up[i] = 0.f;
+                    if (v * 8 >= k) return;
+                    for (int s = 0; s < split0; ++s, src += p.gu_pitch) {
+                        const float4* gp = reinterpret_cast<const float4*>(src);
+                        const float4* upp = reinterpret_cast<const float4*>(src + p.gu_pitch / 2);
+                        const float4 g0 = __ldcg(gp), g1 = __ldcg(gp + 1), u0 = __ldcg(upp), u1 = __ldcg(upp + 1);
+                        h[0] += g0.x; h[1] += g0.y; h[2] += g0.z; h[3] += g0.w; h[4] += g1.x; h[5] += g1.y; h[6] += g1.z; h[7] += g1.w;
+                        up[0] += u0.x; up[1] += u0.y; up[2] += u0.z; up[3] += u0.w; up[4] += u1.x; up[5] += u1.y; up[6] += u1.z; up[7] += u1.w;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) h[i] = v * 8 + i < k ? h[i] / (1.f + expf(-h[i])) * up[i] : 0.f;      // (nobody wrote what is behind)
+                };
+                if constexpr (FMT == FMT_E4M3) {                  // the rows' factors first
+                    for (int at = tid; at < n * row_pieces; at += kMoeBuilders) {
+                        const int j = at / row_pieces, v = at - j * row_pieces;
+                        float h[8];
+                        hidden(j, v, h);
+                        uint32_t top = 0;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const uint32_t b = __float_as_uint(h[i]) & 0x7FFFFFFFu;
+                            if (b < 0x7F800000u) top = max(top, b);
+                        }
+                        top = __reduce_max_sync(0xFFFFFFFFu, top);
+                        if (lane == 0) atomicMax(&sh.slot_top[j], top);
+                    }
+                    builders_sync();
+                }
+                if (tid < n) {
+                    float factor, inv;
+                    moe_row_factor<FMT>(sh.slot_top[tid], factor, inv);
+                    slot_scale[tid] = factor;
+                }
+                for (int at = tid; at < n * row_pieces; at += kMoeBuilders) {
+                    const int j = at / row_pieces, v = at - j * row_pieces;
+                    float h[8], factor, inv;
+                    hidden(j, v, h);
+                    moe_row_factor<FMT>(sh.slot_top[j], factor, inv);
+                    if constexpr (FMT == FMT_E4M3) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) h[i] *= inv;
+                    }
+                    moe_cut<FMT>(h, v, true, tile + j * value_bytes, tile_scales + j * scale_pitch);
+                }
+                fence_proxy_async_smem();                         // visible to the tensor core
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar_of(sh.tile_full[1]));
+                if (*abort_flag) ok = false;
+                ok = __all_sync(0xFFFFFFFFu, ok);
             }
-            if (*abort_flag) ok = false;
-        }
-        if (ph == 0) {
-            __syncthreads();
-            if (threadIdx.x == 0 && sh.run_count[0] > 0 && !*abort_flag) {
-                const MoeRun b = sh.runs[0][sh.run_count[0] - 1];
-                __threadfence();
-                atomicAdd(done + b.expert, static_cast<unsigned>(b.last - b.first));
+            if (!scales_role && !epilogue_role) continue;
+            ok = ok && warp_bounded_wait(bar_of(sh.tile_full[ph]), run & 1, abort_flag, p.status, DEV_TIMEOUT_MMA_FULL);
+            if (!ok) continue;
+            const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
+            if (scales_role) {
+                // rows of scales -> tensor memory: row r of an operand in lane r % 32 of column r / 32, the same in each quarter
+                const int groups = (n * 8 + 31) / 32;             // columns of 32 activations
+                const int token = lane >> 3, part = lane & 7;
+                for (int el = r.first; el < r.last && ok; ++el) {
+                    const int unit = el / split, piece = el - unit * split;
+                    const int kb1 = items[ph] * (piece + 1) / split;
+                    for (int kb = items[ph] * piece / split; kb < kb1; ++kb) {
+                        if (!warp_bounded_wait(bar_of(sh.full[stage]), phase, abort_flag, p.status, DEV_TIMEOUT_MMA_FULL)) { ok = false; break; }
+                        const uint4* rows = reinterpret_cast<const uint4*>(smem_gen + kMoeStageScaleOffset + stage * kMoeStageScales);
+                        uint32_t a[16], b[16];
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            const uint4 s = rows[c * 32 + lane];
+                            if constexpr (FMT == FMT_E4M3) {
+                                a[c] = s.x; a[4 + c] = s.y; a[8 + c] = s.z; a[12 + c] = s.w;
+                            } else {                              // 16 bytes are 512 of K: this stage's half of them
+                                a[c] = kb & 1 ? s.z : s.x; a[4 + c] = kb & 1 ? s.w : s.y; a[8 + c] = a[12 + c] = 0;
+                            }
+                        }
+#pragma unroll
+                        for (int t = 0; t < 4; ++t)
+#pragma unroll
+                            for (int c = 0; c < 4; ++c)
+                                b[t * 4 + c] = t < KT && c < groups && c * 4 + token < n
+                                                   ? *reinterpret_cast<const uint32_t*>(tile_scales + (c * 4 + token) * scale_pitch + (kb * KT + t) * 32 + part * 4)
+                                                   : 0u;
+                        if (!warp_bounded_wait(bar_of(sh.sf_empty[buf]), buf_phase ^ 1u, abort_flag, p.status, DEV_TIMEOUT_MMA_ACC_EMPTY)) { ok = false; break; }
+                        tc_fence_after_sync();
+                        tmem_st_32x16(tmem_base + lanes + kMoeSfBase + buf * 32, a);
+                        tmem_st_32x16(tmem_base + lanes + kMoeSfBase + buf * 32 + 16, b);
+                        tmem_st_wait();
+                        tc_fence_before_sync();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(bar_of(sh.sf_full[buf]));
+                        if (++stage == kMoeStages) { stage = 0; phase ^= 1u; }
+                        buf ^= 1u;
+                        if (buf == 0) buf_phase ^= 1u;
+                    }
+                }
+            } else {
+                const int row = quarter * 32 + lane;              // gate / up: rows 0-63 gate, 64-127 up of 64 channels
+                for (int el = r.first; el < r.last && ok; ++el) {
+                    const int unit = el / split, piece = el - unit * split;
+                    const int channel = ph ? unit * 128 + row : unit * 64 + (row & 63), limit = ph ? p.hidden : p.inter;
+                    const bool in = channel < limit;
+                    float factor = 1.f;
+                    float* out;
+                    size_t step;
+                    if (ph == 0) {
+                        if (in && p.r13) factor = __ldg(p.r13 + (static_cast<size_t>(r.expert) * 2 + (row >> 6)) * p.inter + channel);
+                        out = p.gu + static_cast<size_t>(piece) * p.gu_pitch + (row >> 6) * (p.gu_pitch / 2) + channel;
+                        step = static_cast<size_t>(p.split) * p.gu_pitch;
+                    } else {
+                        if (in && p.r2) factor = __ldg(p.r2 + static_cast<size_t>(r.expert) * p.hidden + channel);
+                        out = p.yp + static_cast<size_t>(piece) * p.y_pitch + channel;
+                        step = static_cast<size_t>(p.split) * p.y_pitch;
+                    }
+                    if (!warp_bounded_wait(bar_of(sh.acc_full[acc]), acc_phase, abort_flag, p.status, DEV_TIMEOUT_EPI_ACC_FULL)) { ok = false; break; }
+                    tc_fence_after_sync();
+                    const uint32_t taddr = tmem_base + lanes + acc * kMoeAccStride;
+                    for (int j = 0; j < n; ++j) {
+                        uint32_t v[8];
+                        tmem_ld_32x8(taddr + j * 8, v);
+                        tmem_ld_wait();
+                        float sum = __uint_as_float(v[kMoeParts - 1]);        // the smallest first
+#pragma unroll
+                        for (int i = kMoeParts - 2; i >= 0; --i) sum += __uint_as_float(v[i]);
+                        if (in) __stcg(out + slot_row[j] * step, sum * factor * slot_scale[j]);
+                    }
+                    tc_fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) {
+                        mbar_arrive(bar_of(sh.acc_empty[acc]));
+                        if (ph == 0) {
+                            __threadfence();
+                            atomicAdd(done + r.expert, 1u);
+                        }
+                    }
+                    acc ^= 1u;
+                    if (acc == 0) acc_phase ^= 1u;
+                }
             }
         }
     }
 
     // ---- all experts' outputs exist: add them up
+    tc_fence_before_sync();
     __syncthreads();
-    if (threadIdx.x == 0 && !*abort_flag) {
+    if (*abort_flag) {
+        const uint64_t t0 = global_timer_ns();                    // copies still in flight land before the CTA leaves
+        while (global_timer_ns() - t0 < 200000ull) {}
+    } else if (threadIdx.x == 0) {
         __threadfence();
         atomicAdd(arrived, 1u);
         const uint64_t t0 = global_timer_ns();
@@ -623,19 +803,21 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_con
         }
     }
     __syncthreads();
-    if (*abort_flag) {
-        // copies still in flight land before the CTA leaves
-        for (; taken < issued; ++taken) {
-            const uint64_t t0 = global_timer_ns();
-            while (!mbar_try_wait(full0 + 8u * (taken % kMoeRing), (taken / kMoeRing) & 1u) && global_timer_ns() - t0 < 20000000ull) {}
-        }
-        return;
+    if (warp == 1) {
+        tc_fence_after_sync();
+        tmem_dealloc(tmem_base, 512);
     }
+    if (*abort_flag) return;
+    const int split1 = sh.split[1];
     for (int at = blockIdx.x * kMoeThreads + threadIdx.x; at < p.tokens * p.hidden; at += gridDim.x * kMoeThreads) {
         const int t = at / p.hidden, c = at - t * p.hidden;
         float sum = 0.f;
-        for (int k = 0; k < p.top; ++k)
-            sum = fmaf(__ldcg(p.weights + t * p.top + k), __ldcg(p.yp + static_cast<size_t>(t * p.top + k) * p.y_pitch + c), sum);
+        for (int i = 0; i < p.top; ++i) {
+            const float* src = p.yp + static_cast<size_t>(t * p.top + i) * p.split * p.y_pitch + c;
+            float y = __ldcg(src);
+            for (int s = 1; s < split1; ++s) y += __ldcg(src + static_cast<size_t>(s) * p.y_pitch);
+            sum = fmaf(__ldcg(p.weights + t * p.top + i), y, sum);
+        }
         p.y[t * p.ldy + c] = BF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(sum)) : __half_as_ushort(__float2half_rn(sum));
     }
 }

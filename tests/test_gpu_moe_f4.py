@@ -35,11 +35,21 @@ class Layer:
         p = np.take_along_axis(z, order, 1)
         return logits, order, p / (p if self.norm else z).sum(1, keepdims=True)
 
+    def left(self, v, dv=0.0):
+        """What six E2M1 numbers may leave of rows of activations (known up to dv)."""
+        a = np.abs(v) + dv
+        n = f4.BLOCK[self.fmt]
+        top = np.pad(a, ((0, 0), (0, -a.shape[1] % n))).reshape(a.shape[0], -1, n).max(-1).repeat(n, 1)[:, :a.shape[1]]
+        return 2.0 ** -14.9 * top + (2.0 ** -17.4 * a.max(1, keepdims=True) if self.fmt == ig.BM_F4_E4M3 else 0.0)
+
     def check(self, y, ids, weights):
         """Errors: an fp32 sum over K is off by at most 2^-23 of the sum of sizes for each of K / 16 + 32 additions (truncated);
-        SiLU moves by at most 1.1 times what its argument does, its evaluation is off by 8 units of 2^-24; the hidden
-        activations are rounded to 11 bits (2^-11 of each, and 2^-39 of the token's largest); then the sum over the
-        choices, and the rounding to the output type."""
+        SiLU moves by at most 1.1 times what its argument does, its evaluation is off by 8 units of 2^-24.  Activations and hidden
+        activations are sums of six E2M1 numbers with block scales.  With scale s = E4M3(amax / 6) the nearest E2M1 number leaves
+        at most s <= 1.0625 amax / 6, a part in 5.6: 5.6^-6 < 2^-14.9 of the block's largest after six; scales below 2^-10 of
+        the row's unit are zero and leave 6 * 2^-10 of it, where the row's largest is 2^10 units or more: 2^-17.4.  With
+        powers of two, amax / s in (3, 6], the first leaves s <= amax / 3 and every further one an eighth: 2^-16.5.  (A block is at most 32
+        long.)  Then the sum over the choices, and the rounding to the output type."""
         logits, order, p = self.select()
         ranked = -np.sort(-logits, 1)
         if self.top < self.E:
@@ -51,14 +61,16 @@ class Layer:
         w13 = f4.values(*f4.quantize(self.plain["w13"].double().numpy(), self.fmt), self.fmt)[:, :self.H]
         w2 = f4.values(*f4.quantize(self.plain["w2"].double().numpy(), self.fmt), self.fmt)[:, :self.I]
         u1, u2 = (self.H / 16 + 32) * 2.0 ** -23, (self.I / 16 + 32) * 2.0 ** -23
+        dx = self.left(x)
         for t in range(self.T):
             for k, e in enumerate(order[t]):
                 a, b = w13[e * 2 * self.I:(e + 1) * 2 * self.I], w2[e * self.H:(e + 1) * self.H]
-                gu, du = a @ x[t], u1 * (np.abs(a) @ np.abs(x[t]))
+                gu, du = a @ x[t], u1 * (np.abs(a) @ np.abs(x[t])) + np.abs(a) @ dx[t]
                 g, u = gu[:self.I], gu[self.I:]
                 s = g / (1 + np.exp(-g))
                 h = s * u
-                dh = 1.1 * du[:self.I] * (np.abs(u) + du[self.I:]) + np.abs(s) * du[self.I:] + np.abs(h) * (2.0 ** -11 + 2.0 ** -21) + np.abs(h).max() * 2.0 ** -39
+                dh = 1.1 * du[:self.I] * (np.abs(u) + du[self.I:]) + np.abs(s) * du[self.I:] + np.abs(h) * 2.0 ** -21
+                dh = dh + self.left(h[None], dh[None])[0]
                 y1, d1 = b @ h, np.abs(b) @ dh + u2 * (np.abs(b) @ np.abs(h))
                 want[t] += p[t, k] * y1
                 bound[t] += p[t, k] * (d1 + 1e-6 * (1 + np.abs(logits).max()) * np.abs(y1))
@@ -106,7 +118,8 @@ def test_ties_go_to_the_lowest_index_and_batches_do_not_change_a_token():
     assert np.array_equal(ids.cpu().numpy(), np.argsort(-rounded, axis=1, kind="stable")[:, :7])
     for t in (0, 7, 19):
         one = layer.run(layer.x[t:t + 1].to(dev()))
-        assert torch.equal(one[1][0], ids[t]) and torch.equal(one[2][0], weights[t]) and torch.equal(one[0][0], y[t])
+        assert torch.equal(one[1][0], ids[t]) and torch.equal(one[2][0], weights[t])
+        assert torch.allclose(one[0][0].float(), y[t].float(), rtol=2.0 ** -6, atol=2.0 ** -10 * y[t].abs().max().item())    # K may be cut differently
 
 
 @pytest.mark.parametrize("scale", [2.0 ** -100, 2.0 ** 100])
