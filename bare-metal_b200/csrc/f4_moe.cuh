@@ -125,7 +125,7 @@ __device__ __forceinline__ void moe_cut(float (&r)[8], int v, bool live, uint8_t
     uint8_t* row = values + (v >> 5) * 1024 + (v & 3) * 4;
     uint8_t* scale = scales + (block >> 2) * 32 + (block & 3);
     const int chunk = (v & 31) >> 2;
-#pragma unroll
+#pragma unroll 1                                                  // (code that runs once waits for its own fetch)
     for (int i = 0; i < kMoeParts; ++i) {
         uint32_t top = 0;                                         // largest |r|: infinities and NaNs are above all numbers
 #pragma unroll
@@ -168,13 +168,44 @@ __device__ __forceinline__ void moe_cut(float (&r)[8], int v, bool live, uint8_t
     }
 }
 
-constexpr int kMoeRouterCtas = 8, kMoeRouterThreads = 512, kMoeRouterTokens = 4;
+constexpr int kMoeRouterCtas = 8, kMoeRouterThreads = 256, kMoeRouterTokens = 4;       // two CTAs an SM: all clusters at once
 
 // order of doubles as unsigned integers, NaN below every number; 0 is left for "no candidate"
 __device__ __forceinline__ unsigned long long logit_key(double v) {
     if (v != v) return 1ull;
     const long long b = __double_as_longlong(v + 0.0);           // -0 counts as +0
     return (b < 0 ? ~static_cast<unsigned long long>(b) : static_cast<unsigned long long>(b) | (1ull << 63)) + 2ull;
+}
+
+// Dot products of one router row with N tokens (those beyond the last: the last again), `AHEAD` pieces of each in flight together (beyond
+// the end the last piece again, not added).
+template <bool BF16, int N, int AHEAD>
+__device__ __forceinline__ void moe_logits(const uint16_t* row, const uint16_t* x, long long ldx, int tokens, int pieces, int lane, double (&sum)[N]) {
+    const uint4* rows[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        rows[j] = reinterpret_cast<const uint4*>(x + min(j, tokens - 1) * ldx);
+        sum[j] = 0.0;
+    }
+#pragma unroll 1
+    for (int v0 = lane; v0 < pieces + lane; v0 += 32 * AHEAD) {
+        uint4 w[AHEAD], d[N][AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            const int v = min(v0 + 32 * i, pieces - 1);
+            w[i] = __ldg(reinterpret_cast<const uint4*>(row) + v);
+#pragma unroll
+            for (int j = 0; j < N; ++j) d[j][i] = __ldg(rows[j] + v);
+        }
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const float s = dot8<BF16>(d[j][i], w[i]);
+                if (v0 + 32 * i < pieces) sum[j] += static_cast<double>(s);
+            }
+        }
+    }
 }
 
 template <int FMT, bool BF16>
@@ -198,34 +229,12 @@ moe_router_kernel(const MoeParams p) {
     for (int e = rank * kWarps + warp; e < p.experts; e += kMoeRouterCtas * kWarps) {
         const uint16_t* row = p.router + static_cast<size_t>(e) * p.hidden;
         double sum[kMoeRouterTokens] = {0.0, 0.0, 0.0, 0.0};
-        if (vec_ok) {
-            // the loads of several pieces in flight together: beyond the end the last piece again, against zeros
-            constexpr int AHEAD = 8;
-            for (int v0 = lane; v0 < pieces; v0 += 32 * AHEAD) {
-                uint4 w[AHEAD];
-#pragma unroll
-                for (int i = 0; i < AHEAD; ++i) {
-                    const int v = v0 + 32 * i;
-                    w[i] = __ldg(reinterpret_cast<const uint4*>(row) + min(v, pieces - 1));
-                    if (v >= pieces) w[i] = make_uint4(0, 0, 0, 0);
-                }
-                for (int j = 0; j < n; ++j) {
-                    const uint4* x = reinterpret_cast<const uint4*>(p.x + (t0 + j) * p.ldx);
-                    uint4 d[AHEAD];
-#pragma unroll
-                    for (int i = 0; i < AHEAD; ++i) {
-                        const int v = v0 + 32 * i;
-                        d[i] = __ldg(x + min(v, pieces - 1));
-                        if (v >= pieces) d[i] = make_uint4(0, 0, 0, 0);
-                    }
-                    double s = 0.0;
-#pragma unroll
-                    for (int i = 0; i < AHEAD; ++i) s += static_cast<double>(dot8<BF16>(d[i], w[i]));
-#pragma unroll
-                    for (int k = 0; k < kMoeRouterTokens; ++k)
-                        if (k == j) sum[k] += s;
-                }
-            }
+        if (vec_ok && n == 1) {
+            double one[1];
+            moe_logits<BF16, 1, 8>(row, p.x + t0 * p.ldx, p.ldx, 1, pieces, lane, one);
+            sum[0] = one[0];
+        } else if (vec_ok) {
+            moe_logits<BF16, kMoeRouterTokens, 3>(row, p.x + t0 * p.ldx, p.ldx, n, pieces, lane, sum);
         } else {
             for (int v = lane; v < pieces; v += 32) {
                 const uint4 w = moe_piece<BF16>(row, v, p.hidden, p.router_vec_ok);
@@ -294,14 +303,16 @@ moe_router_kernel(const MoeParams p) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) key[i] = lane + 32 * i < p.experts ? logit_key(logits[lane + 32 * i]) : 0ull;
     double first = 0.0;
-    float mine = 0.f;                                             // lane r: weight of the r-th choice
+    double mine_logit = 0.0;                                      // lane r: the r-th choice
     int mine_id = 0;
     for (int r = 0; r < p.top; ++r) {
         unsigned long long best = 0ull;
         int at = kMoeMaxExperts;
 #pragma unroll
-        for (int i = 0; i < PER; ++i)
+        for (int i = 0; i < PER; ++i) {
+            if (32 * i >= p.experts) break;
             if (key[i] > best) { best = key[i]; at = lane + 32 * i; }
+        }
         const uint32_t hi = __reduce_max_sync(0xFFFFFFFFu, static_cast<uint32_t>(best >> 32));
         const bool top_hi = static_cast<uint32_t>(best >> 32) == hi;
         const uint32_t lo = __reduce_max_sync(0xFFFFFFFFu, top_hi ? static_cast<uint32_t>(best) : 0u);
@@ -311,8 +322,9 @@ moe_router_kernel(const MoeParams p) {
             if (lane + 32 * i == id) key[i] = 0ull;
         const double v = logits[id];
         if (r == 0) first = v;
-        if (lane == r) { mine = expf(static_cast<float>(v - first)); mine_id = id; }
+        if (lane == r) { mine_logit = v; mine_id = id; }
     }
+    const float mine = expf(static_cast<float>(mine_logit - first));
     float z = lane < p.top ? mine : 0.f;
     if (!p.normalize) {
         z = 0.f;
@@ -330,8 +342,9 @@ moe_router_kernel(const MoeParams p) {
     }
 }
 
-constexpr int kMoeBuilders = 512;                               // warps 2 to 17
-constexpr int kMoeThreads = 64 + kMoeBuilders;                  // TMA producer, MMA issuer, 4 scale warps, 4 epilogue warps, 8 more
+constexpr int kMoeBuilderWarps = 12;
+constexpr int kMoeBuilders = 32 * kMoeBuilderWarps;             // the last warps
+constexpr int kMoeThreads = 10 * 32 + kMoeBuilders;             // TMA producer, MMA issuer, 4 scale warps, 4 epilogue warps, builders
 constexpr int kMoeStages = 4;
 constexpr int kMoeTileTokens = 16;                              // tokens of a pass at most: 128 MMA columns
 constexpr int kMoeTileBytes = 128 * 1024;                       // activations of a pass: 8 tokens of 4096, 16 of 2048
@@ -339,8 +352,10 @@ constexpr int kMoeTileScales = 17 * 1024;
 constexpr int kMoeStageValues = 128 * 128, kMoeStageScales = 128 * 16;
 constexpr int kMoeAccStride = 128, kMoeSfBase = 256;            // tensor memory: two accumulators, two sets of scales (32 columns each)
 
+// Tiles of activations: one, or two halves where a half holds 8 tokens, so that the next is made while one is multiplied.
+__host__ __device__ constexpr int moe_tiles(int k) { return 8 * moe_value_bytes(k) <= kMoeTileBytes / 2 ? 2 : 1; }
 __host__ __device__ constexpr int moe_pass_tokens(int k) {       // an even number
-    const int n = kMoeTileBytes / moe_value_bytes(k);
+    const int n = kMoeTileBytes / moe_tiles(k) / moe_value_bytes(k);
     return n < kMoeTileTokens ? n / 2 * 2 : kMoeTileTokens;
 }
 __host__ __device__ constexpr int moe_tile_scale_pitch(int k, int fmt) { return moe_scale_bytes(k, fmt) + 32; }   // tokens 8 banks apart
@@ -356,12 +371,14 @@ struct MoeShared {
     int start[2][kMoeMaxExperts + 1];            // units x passes before each expert, per phase
     MoeRun runs[2][kMoeMaxRuns];
     int run_count[2], split[2];
-    int slot_row[4][kMoeTileTokens];             // per run (mod 4): assignment (token * top + choice) of each token of the pass
+    uint8_t ids[kMoeMaxTokens * kMoeMaxTop];     // the router's choices
+    float x_scale[kMoeMaxTokens];
+    uint16_t slot_row[4][kMoeTileTokens];        // per run (mod 4): assignment (token * top + choice) of each token of the pass
     float slot_scale[4][kMoeTileTokens];         // what its sums are multiplied with
-    uint32_t slot_top[kMoeTileTokens];           // largest hidden activation, fp32 bits
+    uint32_t slot_top[2][kMoeTileTokens];        // per run (mod 2): largest hidden activation, fp32 bits
     int abort_flag;
     uint32_t tmem_slot;
-    unsigned long long full[kMoeStages], empty[kMoeStages], sf_full[2], sf_empty[2], acc_full[2], acc_empty[2], tile_full[2], tile_empty, drain;
+    unsigned long long full[kMoeStages], empty[kMoeStages], sf_full[2], sf_empty[2], acc_full[2], acc_empty[2], tile_full[2][2], tile_empty[2][2], drain;
 };
 constexpr int kMoeStageScaleOffset = kMoeStages * kMoeStageValues;
 constexpr int kMoeTileOffset = kMoeStageScaleOffset + kMoeStages * kMoeStageScales;
@@ -389,8 +406,8 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_con
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
     MoeShared& sh = *reinterpret_cast<MoeShared*>(smem_gen + kMoeSharedOffset);
-    uint8_t* tile = smem_gen + kMoeTileOffset;
-    uint8_t* tile_scales = smem_gen + kMoeTileScaleOffset;
+    uint8_t* tiles0 = smem_gen + kMoeTileOffset;
+    uint8_t* tile_scales0 = smem_gen + kMoeTileScaleOffset;
     const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     volatile int* abort_flag = &sh.abort_flag;
     unsigned* done = p.counters;
@@ -400,6 +417,7 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_con
     const int units[2] = {(p.inter + 63) / 64, (p.hidden + 127) / 128};
     const int pass_tokens[2] = {moe_pass_tokens(p.hidden), moe_pass_tokens(p.inter)};
     const int items[2] = {moe_k_blocks(p.hidden), moe_k_blocks(p.inter)};
+    const int tiles[2] = {moe_tiles(p.hidden), moe_tiles(p.inter)};
 
     // ---- who does what: token sets of the experts, work before each expert, this CTA's runs
     for (int e = threadIdx.x; e < p.experts; e += kMoeThreads) sh.token_mask[e] = 0ull;
@@ -414,9 +432,12 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_con
             mbar_init(bar_of(sh.acc_full[i]), 1);
             mbar_init(bar_of(sh.acc_empty[i]), 4);
         }
-        mbar_init(bar_of(sh.tile_full[0]), 1);                   // gate / up: copies of what the router kernel cut
-        mbar_init(bar_of(sh.tile_full[1]), kMoeBuilders / 32);   // down: cut here
-        mbar_init(bar_of(sh.tile_empty), 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(bar_of(sh.tile_full[0][i]), 1);                   // gate / up: copies of what the router kernel cut
+            mbar_init(bar_of(sh.tile_full[1][i]), kMoeBuilderWarps);    // down: cut here
+            mbar_init(bar_of(sh.tile_empty[0][i]), 1);
+            mbar_init(bar_of(sh.tile_empty[1][i]), 1);
+        }
         mbar_init(bar_of(sh.drain), 1);
         sh.abort_flag = 0;
         fence_mbar_init();
@@ -429,7 +450,12 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_con
     __syncthreads();
     tc_fence_after_sync();
     const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(&sh.tmem_slot);
-    for (int a = threadIdx.x; a < p.tokens * p.top; a += kMoeThreads) atomicOr(&sh.token_mask[p.ids[a]], 1ull << (a / p.top));
+    for (int a = threadIdx.x; a < p.tokens * p.top; a += kMoeThreads) {
+        const int e = p.ids[a];
+        sh.ids[a] = static_cast<uint8_t>(e);
+        atomicOr(&sh.token_mask[e], 1ull << (a / p.top));
+    }
+    if (static_cast<int>(threadIdx.x) < p.tokens) sh.x_scale[threadIdx.x] = p.x_scale[threadIdx.x];
     __syncthreads();
     if (warp < 2) {
         const int ph = warp;
@@ -495,7 +521,7 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_con
         for (int i = 0; i < r.pass * pass_tokens[ph] + j; ++i) m &= m - 1;
         const int t = __ffsll(static_cast<long long>(m)) - 1;
         int choice = 0;
-        while (choice < p.top - 1 && p.ids[t * p.top + choice] != r.expert) ++choice;
+        while (choice < p.top - 1 && sh.ids[t * p.top + choice] != r.expert) ++choice;
         return t * p.top + choice;
     };
 
@@ -534,7 +560,8 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_con
             const MoeRun r = sh.runs[ph][run];
             const int columns = (run_tokens(r, ph) + 1) / 2 * 16;
             const uint32_t idesc0 = make_idesc_f4<FMT>(128, columns, 0), idesc2 = make_idesc_f4<FMT>(128, columns, 2);
-            if (!warp_bounded_wait(bar_of(sh.tile_full[ph]), run & 1, abort_flag, p.status, DEV_TIMEOUT_MMA_FULL)) { ok = false; break; }
+            const int tile_at = run % tiles[ph], tile_use = run / tiles[ph];
+            if (!warp_bounded_wait(bar_of(sh.tile_full[ph][tile_at]), tile_use & 1, abort_flag, p.status, DEV_TIMEOUT_MMA_FULL)) { ok = false; break; }
             for (int el = r.first; el < r.last && ok; ++el) {
                 const int unit = el / split, piece = el - unit * split;
                 const int kb0 = items[ph] * piece / split, kb1 = items[ph] * (piece + 1) / split;
@@ -547,7 +574,7 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_con
                         const uint32_t d = tmem_base + acc * kMoeAccStride, sfa = tmem_base + kMoeSfBase + buf * 32, sfb = sfa + 16;
                         const uint64_t a_desc = make_smem_desc(smem_base + stage * kMoeStageValues, 0, 1024, SWIZZLE_128B_DESC);
                         // the 8 columns of a token are one row group; the groups lie a token's activations apart
-                        const uint64_t b_desc = make_smem_desc(smem_base + kMoeTileOffset + kb * 1024, 0, items[ph] * 1024, SWIZZLE_128B_DESC);
+                        const uint64_t b_desc = make_smem_desc(smem_base + kMoeTileOffset + tile_at * (kMoeTileBytes / 2) + kb * 1024, 0, items[ph] * 1024, SWIZZLE_128B_DESC);
 #pragma unroll
                         for (int ks = 0; ks < 4; ++ks) {
                             const int t = ks * KT / 4;
@@ -569,7 +596,7 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_con
                 if (acc == 0) acc_phase ^= 1u;
             }
             if (!ok) break;
-            if (elect_one()) tc_commit(bar_of(sh.tile_empty));
+            if (elect_one()) tc_commit(bar_of(sh.tile_empty[ph][tile_at]));
             __syncwarp();
         }
         if (!ok) {
@@ -579,32 +606,36 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_con
             while (!mbar_try_wait(bar_of(sh.drain), 0) && global_timer_ns() - t0 < 20000000ull) {}
         }
     } else {
-        // ------------------------------------------------------------------ builders; among them scale warps and epilogue warps
-        const int quarter = warp & 3, tid = static_cast<int>(threadIdx.x) - 64;
+        // ------------------------------------------------------------------ scale warps, epilogue warps and builders
+        const int quarter = warp & 3, tid = static_cast<int>(threadIdx.x) - 320;
         const bool scales_role = warp < 6, epilogue_role = warp >= 6 && warp < 10;
         uint32_t stage = 0, phase = 0, buf = 0, buf_phase = 0, acc = 0, acc_phase = 0;
-        bool ok = true;                                           // a warp that gave up still meets the others at their barriers
+        bool ok = true;                                           // a builder that gave up still meets the others at their barriers
         for (int it = 0; it < runs; ++it) {
             const int ph = it >= count0, run = ph ? it - count0 : it, split = sh.split[ph], k = ph ? p.inter : p.hidden;
+            const int tile_at = run % tiles[ph], tile_use = run / tiles[ph];
             const MoeRun r = sh.runs[ph][run];
             const int n = run_tokens(r, ph), value_bytes = moe_value_bytes(k), scale_pitch = moe_tile_scale_pitch(k, FMT);
-            int* slot_row = sh.slot_row[it & 3];
+            uint8_t* tile = tiles0 + tile_at * (kMoeTileBytes / 2);
+            uint8_t* tile_scales = tile_scales0 + tile_at * (kMoeTileScales / 2);
+            uint16_t* slot_row = sh.slot_row[it & 3];
             float* slot_scale = sh.slot_scale[it & 3];
-            // the tile of the run before has been read.  The scale and epilogue warps know by their own work up to the last run but one
-            // that it is this phase of the barrier that they look at; the others keep up with every run.
-            if (ph == 1 || (!scales_role && !epilogue_role))
-                ok = ok && (it == 0 || warp_bounded_wait(bar_of(sh.tile_empty), (it - 1) & 1, abort_flag, p.status, DEV_TIMEOUT_PRODUCER_EMPTY));
-            if (ph == 0) {
-                if (warp == 10) {                                 // copies what the router kernel has cut
-                    if (ok) {
-                        const uint32_t bar = bar_of(sh.tile_full[0]);
+            if (!scales_role && !epilogue_role) {
+                // the tile's last use is over (all builders keep up with every run, so a barrier is never two phases ahead)
+                auto wait_empty = [&](int phs, int at, int parity) {
+                    ok = ok && warp_bounded_wait(bar_of(sh.tile_empty[phs][at]), parity, abort_flag, p.status, DEV_TIMEOUT_PRODUCER_EMPTY);
+                };
+                wait_empty(ph, tile_at, (tile_use & 1) ^ 1);
+                if (ph == 0) {
+                    if (warp == 10 && ok) {                       // copies what the router kernel has cut
+                        const uint32_t bar = bar_of(sh.tile_full[0][tile_at]);
                         const int scale_bytes = moe_scale_bytes(k, FMT);
                         int t = 0;
                         if (lane < n) {
                             const int row = slot_of(r, 0, lane);
                             t = row / p.top;
-                            slot_row[lane] = row;
-                            slot_scale[lane] = p.x_scale[t];
+                            slot_row[lane] = static_cast<uint16_t>(row);
+                            slot_scale[lane] = sh.x_scale[t];
                         }
                         __syncwarp();
                         if (lane == 0) mbar_expect_tx(bar, n * (value_bytes + scale_bytes));
@@ -614,12 +645,17 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_con
                             bulk_load(smem_u32(tile_scales) + lane * scale_pitch, p.x_scales + static_cast<size_t>(t) * scale_bytes, scale_bytes, bar);
                         }
                     }
+                    continue;
                 }
-            } else {
                 // ---- hidden activations of the pass: silu(gate) * up from the sums of all CTAs, cut into their parts
+                if (run == 0)                                     // (the tiles of both phases share their memory)
+                    for (int i = 0; i < tiles[0] && i < count0; ++i) {
+                        const int last = (count0 - 1 - i) / tiles[0];     // use of the tile that run count0 - 1 - i had
+                        wait_empty(0, (count0 - 1 - i) % tiles[0], last & 1);
+                    }
                 if (tid < n) {
-                    slot_row[tid] = slot_of(r, 1, tid);
-                    sh.slot_top[tid] = 0u;
+                    slot_row[tid] = static_cast<uint16_t>(slot_of(r, 1, tid));
+                    sh.slot_top[run & 1][tid] = 0u;
                 }
                 if (tid == 32) {
                     const unsigned want = static_cast<unsigned>(sh.start[0][r.expert + 1] - sh.start[0][r.expert]) * sh.split[0] * 4u;
@@ -635,14 +671,16 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_con
                     }
                 }
                 builders_sync();
-                const int row_pieces = items[1] * (kF4BK / 8);    // a multiple of 32: a warp's pieces are one token's
+                // a warp takes 256 activations of a token at a time: 1 KiB of the tile, in fp32 as well as cut up
                 const int split0 = sh.split[0];
-                auto hidden = [&](int j, int v, float (&h)[8]) {
+                auto hidden = [&](int j, int kb, float (&h)[8]) {
+                    const int v = kb * 32 + lane;
                     const float* src = p.gu + static_cast<size_t>(slot_row[j]) * p.split * p.gu_pitch + v * 8;
                     float up[8];
 #pragma unroll
                     for (int i = 0; i < 8; ++i) h[i] = up[i] = 0.f;
                     if (v * 8 >= k) return;
+#pragma unroll 1
                     for (int s = 0; s < split0; ++s, src += p.gu_pitch) {
                         const float4* gp = reinterpret_cast<const float4*>(src);
                         const float4* upp = reinterpret_cast<const float4*>(src + p.gu_pitch / 2);
@@ -653,46 +691,55 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_con
 #pragma unroll
                     for (int i = 0; i < 8; ++i) h[i] = v * 8 + i < k ? h[i] / (1.f + expf(-h[i])) * up[i] : 0.f;      // (nobody wrote what is behind)
                 };
-                if constexpr (FMT == FMT_E4M3) {                  // the rows' factors first
-                    for (int at = tid; at < n * row_pieces; at += kMoeBuilders) {
-                        const int j = at / row_pieces, v = at - j * row_pieces;
+                if constexpr (FMT == FMT_E4M3) {                  // the rows' factors first; the numbers wait in the tile
+#pragma unroll 1
+                    for (int at = warp - 10; at < n * items[1]; at += kMoeBuilderWarps) {
+                        const int j = at / items[1], kb = at - j * items[1];
                         float h[8];
-                        hidden(j, v, h);
+                        hidden(j, kb, h);
                         uint32_t top = 0;
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
                             const uint32_t b = __float_as_uint(h[i]) & 0x7FFFFFFFu;
                             if (b < 0x7F800000u) top = max(top, b);
                         }
+                        float4* keep = reinterpret_cast<float4*>(tile + j * value_bytes + kb * 1024) + lane;
+                        keep[0] = make_float4(h[0], h[1], h[2], h[3]);
+                        keep[32] = make_float4(h[4], h[5], h[6], h[7]);
                         top = __reduce_max_sync(0xFFFFFFFFu, top);
-                        if (lane == 0) atomicMax(&sh.slot_top[j], top);
+                        if (lane == 0) atomicMax(&sh.slot_top[run & 1][j], top);
                     }
                     builders_sync();
                 }
                 if (tid < n) {
                     float factor, inv;
-                    moe_row_factor<FMT>(sh.slot_top[tid], factor, inv);
+                    moe_row_factor<FMT>(sh.slot_top[run & 1][tid], factor, inv);
                     slot_scale[tid] = factor;
                 }
-                for (int at = tid; at < n * row_pieces; at += kMoeBuilders) {
-                    const int j = at / row_pieces, v = at - j * row_pieces;
-                    float h[8], factor, inv;
-                    hidden(j, v, h);
-                    moe_row_factor<FMT>(sh.slot_top[j], factor, inv);
+#pragma unroll 1
+                for (int at = warp - 10; at < n * items[1]; at += kMoeBuilderWarps) {
+                    const int j = at / items[1], kb = at - j * items[1];
+                    float h[8];
                     if constexpr (FMT == FMT_E4M3) {
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) h[i] *= inv;
+                        float factor, inv;
+                        moe_row_factor<FMT>(sh.slot_top[run & 1][j], factor, inv);
+                        const float4* keep = reinterpret_cast<const float4*>(tile + j * value_bytes + kb * 1024) + lane;
+                        const float4 lo = keep[0], hi = keep[32];
+                        h[0] = lo.x * inv; h[1] = lo.y * inv; h[2] = lo.z * inv; h[3] = lo.w * inv;
+                        h[4] = hi.x * inv; h[5] = hi.y * inv; h[6] = hi.z * inv; h[7] = hi.w * inv;
+                        __syncwarp();                             // all lanes have theirs: the cut numbers take the place
+                    } else {
+                        hidden(j, kb, h);
                     }
-                    moe_cut<FMT>(h, v, true, tile + j * value_bytes, tile_scales + j * scale_pitch);
+                    moe_cut<FMT>(h, kb * 32 + lane, true, tile + j * value_bytes, tile_scales + j * scale_pitch);
                 }
                 fence_proxy_async_smem();                         // visible to the tensor core
                 __syncwarp();
-                if (lane == 0) mbar_arrive(bar_of(sh.tile_full[1]));
-                if (*abort_flag) ok = false;
-                ok = __all_sync(0xFFFFFFFFu, ok);
+                if (lane == 0) mbar_arrive(bar_of(sh.tile_full[1][tile_at]));
+                ok = __all_sync(0xFFFFFFFFu, ok && *abort_flag == 0);
+                continue;
             }
-            if (!scales_role && !epilogue_role) continue;
-            ok = ok && warp_bounded_wait(bar_of(sh.tile_full[ph]), run & 1, abort_flag, p.status, DEV_TIMEOUT_MMA_FULL);
+            ok = ok && warp_bounded_wait(bar_of(sh.tile_full[ph][tile_at]), tile_use & 1, abort_flag, p.status, DEV_TIMEOUT_MMA_FULL);
             if (!ok) continue;
             const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
             if (scales_role) {
@@ -808,17 +855,41 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_con
         tmem_dealloc(tmem_base, 512);
     }
     if (*abort_flag) return;
-    const int split1 = sh.split[1];
-    for (int at = blockIdx.x * kMoeThreads + threadIdx.x; at < p.tokens * p.hidden; at += gridDim.x * kMoeThreads) {
-        const int t = at / p.hidden, c = at - t * p.hidden;
-        float sum = 0.f;
-        for (int i = 0; i < p.top; ++i) {
-            const float* src = p.yp + static_cast<size_t>(t * p.top + i) * p.split * p.y_pitch + c;
-            float y = __ldcg(src);
-            for (int s = 1; s < split1; ++s) y += __ldcg(src + static_cast<size_t>(s) * p.y_pitch);
-            sum = fmaf(__ldcg(p.weights + t * p.top + i), y, sum);
+    const int split1 = sh.split[1], quads = (p.hidden + 3) / 4;
+    for (int at = blockIdx.x * kMoeThreads + threadIdx.x; at < p.tokens * quads; at += gridDim.x * kMoeThreads) {
+        const int t = at / quads, c = (at - t * quads) * 4;      // (the rows of the sums are whole 32s long)
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int i0 = 0; i0 < p.top; i0 += 4) {                   // four choices' loads in flight
+            float4 y[4];
+            float weight[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int row = t * p.top + min(i0 + i, p.top - 1);
+                y[i] = __ldcg(reinterpret_cast<const float4*>(p.yp + static_cast<size_t>(row) * p.split * p.y_pitch + c));
+                weight[i] = __ldcg(p.weights + row);
+            }
+            for (int s = 1; s < split1; ++s)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int row = t * p.top + min(i0 + i, p.top - 1);
+                    const float4 more = __ldcg(reinterpret_cast<const float4*>(p.yp + (static_cast<size_t>(row) * p.split + s) * p.y_pitch + c));
+                    y[i].x += more.x; y[i].y += more.y; y[i].z += more.z; y[i].w += more.w;
+                }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (i0 + i >= p.top) break;
+                sum.x = fmaf(weight[i], y[i].x, sum.x);
+                sum.y = fmaf(weight[i], y[i].y, sum.y);
+                sum.z = fmaf(weight[i], y[i].z, sum.z);
+                sum.w = fmaf(weight[i], y[i].w, sum.w);
+            }
         }
-        p.y[t * p.ldy + c] = BF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(sum)) : __half_as_ushort(__float2half_rn(sum));
+        const uint32_t lo = float_to_pair<BF16>(sum.x, sum.y), hi = float_to_pair<BF16>(sum.z, sum.w);
+        uint16_t* dst = p.y + t * p.ldy + c;
+        dst[0] = static_cast<uint16_t>(lo);
+        if (c + 1 < p.hidden) dst[1] = static_cast<uint16_t>(lo >> 16);
+        if (c + 2 < p.hidden) dst[2] = static_cast<uint16_t>(hi);
+        if (c + 3 < p.hidden) dst[3] = static_cast<uint16_t>(hi >> 16);
     }
 }
 
