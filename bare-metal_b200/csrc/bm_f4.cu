@@ -202,17 +202,20 @@ static int launch_moe(const CUtensorMap& w13, const CUtensorMap& s13, const CUte
     auto kern = moe_experts_kernel<FMT, BF16>;
     static ConfiguredFlags flags;
     if (int rc = ensure_smem_limit(flags, kern, kMoeSmemBytes)) return rc;
-    BM_CUDA_TRY(launch_pdl(moe_router_kernel<FMT, BF16>, dim3(clusters * kMoeRouterCtas), dim3(kMoeRouterThreads), 0, stream, kMoeRouterCtas, p));
+    BM_CUDA_TRY(launch_pdl(moe_router_kernel<FMT, BF16>, dim3(clusters * kMoeRouterCtas), dim3(kMoeRouterThreads),
+                           sizeof(double) * kMoeRouterChunks * p.experts, stream, kMoeRouterCtas, p));
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(ctas);
     cfg.blockDim = dim3(kMoeThreads);
     cfg.dynamicSmemBytes = kMoeSmemBytes;
     cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeCooperative;             // its CTAs wait for one another
     attr[0].val.cooperative = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = opt(OPT_PDL) != 0 ? 2 : 1;
     BM_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, w13, s13, w2, s2, p));
     return BM_OK;
 }
@@ -383,9 +386,7 @@ int bm_moe_f4(const void* X, const void* router, int x_type, const uint8_t* W13,
     p.split = w.split;
     p.y_pitch = w.y_pitch;
     p.status = dev->status;
-    int clusters = T < 16 ? T : 16;                          // 128 CTAs
-    p.tokens_per_cluster = ceil_div(T, clusters);
-    clusters = ceil_div(T, p.tokens_per_cluster);
+    const int clusters = 2 * ceil_div(T, kMoeRouterTokens);  // at most 128 CTAs
     CUtensorMap mw13, ms13, mw2, ms2;
     if (int rc = expert_maps(&mw13, &ms13, W13, S13, 2 * E, I, H, format, 2)) return rc;
     if (int rc = expert_maps(&mw2, &ms2, W2, S2, E, H, I, format, 1)) return rc;

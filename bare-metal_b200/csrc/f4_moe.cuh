@@ -66,7 +66,6 @@ struct MoeParams {
     const float* r2;
     int tokens, hidden, inter, experts, top;
     int normalize;
-    int tokens_per_cluster;
     int x_vec_ok, router_vec_ok;
     unsigned* counters;
     int counter_words;
@@ -93,19 +92,6 @@ __device__ __forceinline__ uint4 moe_piece(const uint16_t* row, int v, int k, bo
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-template <bool BF16>
-__device__ __forceinline__ float dot8(const uint4& a, const uint4& b) {
-    const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
-    float s = 0.f;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const float2 p = pair_to_float<BF16>(x[j]), q = pair_to_float<BF16>(y[j]);
-        s = fmaf(p.x, q.x, s);
-        s = fmaf(p.y, q.y, s);
-    }
-    return s;
-}
-
 // FMT_E4M3: the power of two that puts a row with largest |v| = top (fp32 bits) where the quantiser puts it, and its inverse
 template <int FMT>
 __device__ __forceinline__ void moe_row_factor(uint32_t top_bits, float& factor, float& inv) {
@@ -125,14 +111,18 @@ __device__ __forceinline__ void moe_cut(float (&r)[8], int v, bool live, uint8_t
     uint8_t* row = values + (v >> 5) * 1024 + (v & 3) * 4;
     uint8_t* scale = scales + (block >> 2) * 32 + (block & 3);
     const int chunk = (v & 31) >> 2;
+    float odd = 0.f;                                              // a NaN where one of the block's numbers is none
+#pragma unroll
+    for (int j = 0; j < 8; ++j) odd = fmaf(r[j], 0.f, odd);
+#pragma unroll
+    for (int o = 1; o < SHARE; o <<= 1) odd += __shfl_xor_sync(0xFFFFFFFFu, odd, o);
 #pragma unroll 1                                                  // (code that runs once waits for its own fetch)
     for (int i = 0; i < kMoeParts; ++i) {
-        uint32_t top = 0;                                         // largest |r|: infinities and NaNs are above all numbers
+        float top = fmaxf(fmaxf(fmaxf(fabsf(r[0]), fabsf(r[1])), fmaxf(fabsf(r[2]), fabsf(r[3]))),
+                          fmaxf(fmaxf(fabsf(r[4]), fabsf(r[5])), fmaxf(fabsf(r[6]), fabsf(r[7]))));
 #pragma unroll
-        for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(r[j]) & 0x7FFFFFFFu);
-#pragma unroll
-        for (int o = 1; o < SHARE; o <<= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-        const float sixth = __uint_as_float(top) * 0.16666667f;
+        for (int o = 1; o < SHARE; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+        const float sixth = top * 0.16666667f;
         uint32_t byte;
         float s, inv;
         if constexpr (FMT == FMT_E4M3) {
@@ -142,33 +132,84 @@ __device__ __forceinline__ void moe_cut(float (&r)[8], int v, bool live, uint8_t
         } else {
             // the smallest power of two that holds the largest below 6 (or a rounding above it)
             const uint32_t b = __float_as_uint(sixth);
-            byte = min((b >> 23) + ((b & 0x007FFFFFu) != 0 ? 1u : 0u), 253u);
+            byte = min((b + 0x007FFFFFu) >> 23, 253u);
             s = e8m0_value(byte);
             inv = __uint_as_float((254u - byte) << 23);
         }
-        const bool odd = top >= 0x7F800000u;
-        if (odd) byte = FMT == FMT_E4M3 ? 127u : 255u;
         float y[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] = odd ? 0.f : r[j] * inv;
+        for (int j = 0; j < 8; ++j) y[j] = r[j] * inv;
         const uint32_t codes = e2m1x8(y);
         if (live) {
             *reinterpret_cast<uint32_t*>(row + i * 128 + ((chunk ^ i) << 4)) = codes;
-            if (v % SHARE == 0) scale[i * 4] = static_cast<uint8_t>(byte);
+            if (v % SHARE == 0) scale[i * 4] = static_cast<uint8_t>(odd == 0.f ? byte : FMT == FMT_E4M3 ? 127u : 255u);
         }
         uint32_t h[4];
         e2m1x8_to_small_half(codes, h);
         constexpr int kOrder[4] = {1, 3, 0, 2};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const float2 f = pair_to_float<false>(h[j]);
-            r[kOrder[j]] = fmaf(f.x * -16384.f, s, r[kOrder[j]]);
-            r[kOrder[j] + 4] = fmaf(f.y * -16384.f, s, r[kOrder[j] + 4]);
+            const __half2 whole = __hmul2(*reinterpret_cast<const __half2*>(&h[j]), __float2half2_rn(16384.f));
+            const float2 f = __half22float2(whole);
+            r[kOrder[j]] = fmaf(-f.x, s, r[kOrder[j]]);
+            r[kOrder[j] + 4] = fmaf(-f.y, s, r[kOrder[j] + 4]);
         }
     }
 }
 
-constexpr int kMoeRouterCtas = 8, kMoeRouterThreads = 256, kMoeRouterTokens = 4;       // two CTAs an SM: all clusters at once
+// Clusters of 8 CTAs: the first ones choose the experts of up to 8 tokens each, the others cut these tokens up (a CTA per token).
+constexpr int kMoeRouterCtas = 8, kMoeRouterThreads = 256, kMoeRouterTokens = 8;
+constexpr int kMoeRouterChunks = 16;                             // pieces of K that the logits are added up from
+
+template <bool BF16>
+__device__ __forceinline__ void mma_16x8x16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    if constexpr (BF16)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+            : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+            : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+
+// Logits of 16 experts (rows a0 and a1 of lane group g: experts g and g + 8) and 8 tokens over pieces [v0, v1) of 8 of K.  Lane (g, q) holds
+// the 8 numbers of piece 4 i + q of its rows and of token g: any order of K serves an MMA if both operands keep it.  An
+// MMA's 16 products are added in fp32, its results in 64 bits: which expert a token gets must not depend on a sum's rounding.
+template <bool BF16, bool VEC>
+__device__ __forceinline__ void moe_logits(const uint16_t* a0, const uint16_t* a1, const uint16_t* x, int k, int v0, int v1, int q, double (&sum)[4]) {
+    constexpr int AHEAD = 4;                                      // MMA pairs (32 of K) whose loads are in flight together
+#pragma unroll 1
+    for (int v = v0; v < v1; v += 4 * AHEAD) {
+        uint4 a[AHEAD], c[AHEAD], b[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            const int at = v + 4 * i + q;
+            a[i] = c[i] = b[i] = make_uint4(0, 0, 0, 0);
+            if (at < v1) {
+                if constexpr (VEC) {
+                    a[i] = __ldg(reinterpret_cast<const uint4*>(a0) + at);
+                    c[i] = __ldg(reinterpret_cast<const uint4*>(a1) + at);
+                    b[i] = __ldg(reinterpret_cast<const uint4*>(x) + at);
+                } else {
+                    a[i] = moe_piece<BF16>(a0, at, k, false);
+                    c[i] = moe_piece<BF16>(a1, at, k, false);
+                    b[i] = moe_piece<BF16>(x, at, k, false);
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            float d[4];
+            mma_16x8x16<BF16>(d, a[i].x, c[i].x, a[i].y, c[i].y, b[i].x, b[i].y);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sum[j] += static_cast<double>(d[j]);
+            mma_16x8x16<BF16>(d, a[i].z, c[i].z, a[i].w, c[i].w, b[i].z, b[i].w);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sum[j] += static_cast<double>(d[j]);
+        }
+    }
+}
 
 // order of doubles as unsigned integers, NaN below every number; 0 is left for "no candidate"
 __device__ __forceinline__ unsigned long long logit_key(double v) {
@@ -177,114 +218,47 @@ __device__ __forceinline__ unsigned long long logit_key(double v) {
     return (b < 0 ? ~static_cast<unsigned long long>(b) : static_cast<unsigned long long>(b) | (1ull << 63)) + 2ull;
 }
 
-// Dot products of one router row with N tokens (those beyond the last: the last again), `AHEAD` pieces of each in flight together (beyond
-// the end the last piece again, not added).
-template <bool BF16, int N, int AHEAD>
-__device__ __forceinline__ void moe_logits(const uint16_t* row, const uint16_t* x, long long ldx, int tokens, int pieces, int lane, double (&sum)[N]) {
-    const uint4* rows[N];
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-        rows[j] = reinterpret_cast<const uint4*>(x + min(j, tokens - 1) * ldx);
-        sum[j] = 0.0;
-    }
-#pragma unroll 1
-    for (int v0 = lane; v0 < pieces + lane; v0 += 32 * AHEAD) {
-        uint4 w[AHEAD], d[N][AHEAD];
-#pragma unroll
-        for (int i = 0; i < AHEAD; ++i) {
-            const int v = min(v0 + 32 * i, pieces - 1);
-            w[i] = __ldg(reinterpret_cast<const uint4*>(row) + v);
-#pragma unroll
-            for (int j = 0; j < N; ++j) d[j][i] = __ldg(rows[j] + v);
-        }
-#pragma unroll
-        for (int i = 0; i < AHEAD; ++i) {
-#pragma unroll
-            for (int j = 0; j < N; ++j) {
-                const float s = dot8<BF16>(d[j][i], w[i]);
-                if (v0 + 32 * i < pieces) sum[j] += static_cast<double>(s);
-            }
-        }
-    }
-}
-
 template <int FMT, bool BF16>
 __global__ void __launch_bounds__(kMoeRouterThreads)
 moe_router_kernel(const MoeParams p) {
-    __shared__ double logits[kMoeMaxExperts];
     constexpr int kWarps = kMoeRouterThreads / 32;
+    extern __shared__ double parts[];                             // [chunk][expert] of this CTA's token
+    __shared__ double logits[kMoeMaxExperts];
     __shared__ uint32_t warp_max[kWarps];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = static_cast<int>(cluster_ctarank());
-    const int t0 = blockIdx.x / kMoeRouterCtas * p.tokens_per_cluster;
-    const int left = p.tokens - t0, n = left < p.tokens_per_cluster ? left : p.tokens_per_cluster;
+    const int groups = (p.tokens + kMoeRouterTokens - 1) / kMoeRouterTokens;
+    const int cluster = blockIdx.x / kMoeRouterCtas, group = cluster < groups ? cluster : cluster - groups;
+    const int t0 = group * kMoeRouterTokens, n = min(p.tokens - t0, kMoeRouterTokens);
+    const int t = t0 + rank;                                      // the token this CTA selects for, or cuts up
+    const int pieces = (p.hidden + 7) / 8;
     pdl_launch_dependents();
     pdl_wait_prior_grid();        // the call before may still be using the workspace
-    if (blockIdx.x == 0)
-        for (int i = threadIdx.x; i < p.counter_words; i += kMoeRouterThreads) p.counters[i] = 0u;
-    const int pieces = (p.hidden + 7) / 8;
-    const bool vec_ok = p.x_vec_ok && p.router_vec_ok && p.hidden % 8 == 0;
-    cluster_arrive();             // every CTA of the cluster runs: its shared memory may be written
-    cluster_wait();
-    for (int e = rank * kWarps + warp; e < p.experts; e += kMoeRouterCtas * kWarps) {
-        const uint16_t* row = p.router + static_cast<size_t>(e) * p.hidden;
-        double sum[kMoeRouterTokens] = {0.0, 0.0, 0.0, 0.0};
-        if (vec_ok && n == 1) {
-            double one[1];
-            moe_logits<BF16, 1, 8>(row, p.x + t0 * p.ldx, p.ldx, 1, pieces, lane, one);
-            sum[0] = one[0];
-        } else if (vec_ok) {
-            moe_logits<BF16, kMoeRouterTokens, 3>(row, p.x + t0 * p.ldx, p.ldx, n, pieces, lane, sum);
-        } else {
-            for (int v = lane; v < pieces; v += 32) {
-                const uint4 w = moe_piece<BF16>(row, v, p.hidden, p.router_vec_ok);
-#pragma unroll
-                for (int j = 0; j < kMoeRouterTokens; ++j)
-                    if (j < n) sum[j] += static_cast<double>(dot8<BF16>(moe_piece<BF16>(p.x + (t0 + j) * p.ldx, v, p.hidden, p.x_vec_ok), w));
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < kMoeRouterTokens; ++j) {
-            if (j >= n) break;
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) sum[j] += __shfl_xor_sync(0xFFFFFFFFu, sum[j], o);
-            if (lane == 0)
-                asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(mapa_shared(smem_u32(logits + e), j)), "d"(sum[j]) : "memory");
-        }
-    }
-    // token t0 + rank % 4 is cut up by CTAs rank % 4 and rank % 4 + 4, half of its pieces each
-    const int mine_j = rank & 3, x_pieces = moe_k_blocks(p.hidden) * (kF4BK / 8);
-    const bool cuts = mine_j < n;
-    const uint16_t* x_row = p.x + (t0 + mine_j) * p.ldx;
-    if (FMT == FMT_E4M3 && cuts) {
-        uint32_t m = 0;
-        for (int v = threadIdx.x; v < pieces; v += kMoeRouterThreads) {
-            const uint4 d = moe_piece<BF16>(x_row, v, p.hidden, p.x_vec_ok);
-            const uint32_t b = __vmaxu2(__vmaxu2(d.x & 0x7FFF7FFFu, d.y & 0x7FFF7FFFu), __vmaxu2(d.z & 0x7FFF7FFFu, d.w & 0x7FFF7FFFu));
-            m = max(m, max(b & 0xFFFFu, b >> 16));
-        }
-        m = __reduce_max_sync(0xFFFFFFFFu, m);
-        if (lane == 0) warp_max[warp] = m;
-    }
-    cluster_arrive();
-    cluster_wait();
-    if (cuts && warp != 0) {
+    if (cluster >= groups) {
+        // ------------------------------------------------------------------ a token's activations cut up
+        if (rank >= n) return;
+        const uint16_t* row = p.x + t * p.ldx;
         float factor = 1.f, inv = 1.f;
         if (FMT == FMT_E4M3) {
             uint32_t m = 0;
+#pragma unroll 2
+            for (int v = threadIdx.x; v < pieces; v += kMoeRouterThreads) {
+                const uint4 d = moe_piece<BF16>(row, v, p.hidden, p.x_vec_ok);
+                const uint32_t b = __vmaxu2(__vmaxu2(d.x & 0x7FFF7FFFu, d.y & 0x7FFF7FFFu), __vmaxu2(d.z & 0x7FFF7FFFu, d.w & 0x7FFF7FFFu));
+                m = max(m, max(b & 0xFFFFu, b >> 16));
+            }
+            m = __reduce_max_sync(0xFFFFFFFFu, m);
+            if (lane == 0) warp_max[warp] = m;
+            __syncthreads();
             for (int w = 0; w < kWarps; ++w) m = max(m, warp_max[w]);
             const float top = BF16 ? __uint_as_float(m << 16) : __half2float(__ushort_as_half(static_cast<unsigned short>(m)));
             moe_row_factor<FMT>(__float_as_uint(top), factor, inv);
         }
-        const int t = t0 + mine_j, half = rank >> 2;
-        if (half == 0 && threadIdx.x == 32) p.x_scale[t] = factor;
+        if (threadIdx.x == 0) p.x_scale[t] = factor;
         uint8_t* values = p.x_values + static_cast<size_t>(t) * moe_value_bytes(p.hidden);
         uint8_t* scales = p.x_scales + static_cast<size_t>(t) * moe_scale_bytes(p.hidden, FMT);
-        const int first = half * (x_pieces / 2);
-        for (int v0 = first + (warp - 1) * 32; v0 < first + x_pieces / 2; v0 += (kWarps - 1) * 32) {
-            const int v = v0 + lane;                              // (x_pieces / 2 is a multiple of 16)
-            const bool live = v < first + x_pieces / 2;
-            const uint4 d = live ? moe_piece<BF16>(x_row, v, p.hidden, p.x_vec_ok) : make_uint4(0, 0, 0, 0);
+        for (int v = threadIdx.x; v < moe_k_blocks(p.hidden) * (kF4BK / 8); v += kMoeRouterThreads) {      // whole warps
+            const uint4 d = moe_piece<BF16>(row, v, p.hidden, p.x_vec_ok);
             const uint32_t w[4] = {d.x, d.y, d.z, d.w};
             float f[8];
 #pragma unroll
@@ -293,11 +267,46 @@ moe_router_kernel(const MoeParams p) {
                 f[2 * j] = two.x * inv;
                 f[2 * j + 1] = two.y * inv;
             }
-            moe_cut<FMT>(f, v, live, values, scales);
+            moe_cut<FMT>(f, v, true, values, scales);
+        }
+        return;
+    }
+    // ---------------------------------------------------------------------- the choice of experts
+    if (blockIdx.x == 0)
+        for (int i = threadIdx.x; i < p.counter_words; i += kMoeRouterThreads) p.counters[i] = 0u;
+    cluster_arrive();             // every CTA of the cluster runs: its shared memory may be written
+    cluster_wait();
+    {
+        const bool vec_ok = p.x_vec_ok && p.router_vec_ok;        // (the router's rows are whole pieces then)
+        const int g = lane >> 2, q = lane & 3, tiles = (p.experts + 15) / 16, chunk = (pieces + 4 * kMoeRouterChunks - 1) / (4 * kMoeRouterChunks) * 4;
+        const uint16_t* x = p.x + (t0 + min(g, n - 1)) * p.ldx;
+        for (int task = rank * kWarps + warp; task < tiles * kMoeRouterChunks; task += kMoeRouterCtas * kWarps) {
+            const int tile = task / kMoeRouterChunks, c = task % kMoeRouterChunks;
+            const uint16_t* a0 = p.router + static_cast<size_t>(min(tile * 16 + g, p.experts - 1)) * p.hidden;
+            const uint16_t* a1 = p.router + static_cast<size_t>(min(tile * 16 + g + 8, p.experts - 1)) * p.hidden;
+            double sum[4] = {0.0, 0.0, 0.0, 0.0};
+            const int v0 = min(c * chunk, pieces), v1 = min(v0 + chunk, pieces);
+            if (vec_ok) moe_logits<BF16, true>(a0, a1, x, p.hidden, v0, v1, q, sum);
+            else moe_logits<BF16, false>(a0, a1, x, p.hidden, v0, v1, q, sum);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {                         // (expert g, tokens 2q, 2q + 1), (expert g + 8, the same)
+                const int token = q * 2 + (j & 1), e = tile * 16 + g + (j >> 1) * 8;
+                if (token < n && e < p.experts)
+                    asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(mapa_shared(smem_u32(parts + c * p.experts + e), token)), "d"(sum[j]) : "memory");
+            }
         }
     }
-    if (rank >= n || warp != 0) return;                           // this CTA's first warp selects for token t0 + rank
-    const int t = t0 + rank;
+    cluster_arrive();
+    cluster_wait();
+    if (rank >= n) return;
+    for (int e = threadIdx.x; e < p.experts; e += kMoeRouterThreads) {
+        double sum = 0.0;
+#pragma unroll
+        for (int c = 0; c < kMoeRouterChunks; ++c) sum += parts[c * p.experts + e];
+        logits[e] = sum;
+    }
+    __syncthreads();
+    if (warp != 0) return;
     constexpr int PER = kMoeMaxExperts / 32;
     unsigned long long key[PER];
 #pragma unroll
@@ -342,7 +351,10 @@ moe_router_kernel(const MoeParams p) {
     }
 }
 
-constexpr int kMoeBuilderWarps = 12;
+#ifndef BM_MOE_BUILDERS
+#define BM_MOE_BUILDERS 12
+#endif
+constexpr int kMoeBuilderWarps = BM_MOE_BUILDERS;
 constexpr int kMoeBuilders = 32 * kMoeBuilderWarps;             // the last warps
 constexpr int kMoeThreads = 10 * 32 + kMoeBuilders;             // TMA producer, MMA issuer, 4 scale warps, 4 epilogue warps, builders
 constexpr int kMoeStages = 4;
@@ -414,6 +426,12 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_con
     unsigned* arrived = p.counters + p.experts;
     auto bar_of = [&](const unsigned long long& b) { return smem_u32(&b); };
 
+    if (warp == 0 && elect_one()) {
+        prefetch_tensormap(&map_w13);
+        prefetch_tensormap(&map_s13);
+        prefetch_tensormap(&map_w2);
+        prefetch_tensormap(&map_s2);
+    }
     const int units[2] = {(p.inter + 63) / 64, (p.hidden + 127) / 128};
     const int pass_tokens[2] = {moe_pass_tokens(p.hidden), moe_pass_tokens(p.inter)};
     const int items[2] = {moe_k_blocks(p.hidden), moe_k_blocks(p.inter)};
@@ -450,6 +468,8 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_con
     __syncthreads();
     tc_fence_after_sync();
     const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(&sh.tmem_slot);
+    pdl_launch_dependents();
+    pdl_wait_prior_grid();        // what the router kernel wrote
     for (int a = threadIdx.x; a < p.tokens * p.top; a += kMoeThreads) {
         const int e = p.ids[a];
         sh.ids[a] = static_cast<uint8_t>(e);
@@ -484,8 +504,8 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_con
             sh.split[ph] = split;
         }
         __syncwarp();
-        const long long total = static_cast<long long>(carry) * split;
-        const int from = static_cast<int>(total * blockIdx.x / gridDim.x), to = static_cast<int>(total * (blockIdx.x + 1) / gridDim.x);
+        const unsigned total = static_cast<unsigned>(carry) * split, share = total / gridDim.x, rest = total - share * gridDim.x;
+        const int from = static_cast<int>(share * blockIdx.x + min(blockIdx.x, rest)), to = from + static_cast<int>(share + (blockIdx.x < rest ? 1u : 0u));
         int count = 0;
         for (int e0 = 0; e0 < p.experts; e0 += 32) {
             const int e = e0 + lane;
@@ -689,7 +709,7 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_con
                         up[0] += u0.x; up[1] += u0.y; up[2] += u0.z; up[3] += u0.w; up[4] += u1.x; up[5] += u1.y; up[6] += u1.z; up[7] += u1.w;
                     }
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) h[i] = v * 8 + i < k ? h[i] / (1.f + expf(-h[i])) * up[i] : 0.f;      // (nobody wrote what is behind)
+                    for (int i = 0; i < 8; ++i) h[i] = v * 8 + i < k ? __fdividef(h[i], 1.f + expf(-h[i])) * up[i] : 0.f;      // (nobody wrote what is behind)
                 };
                 if constexpr (FMT == FMT_E4M3) {                  // the rows' factors first; the numbers wait in the tile
 #pragma unroll 1
@@ -855,38 +875,42 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_con
         tmem_dealloc(tmem_base, 512);
     }
     if (*abort_flag) return;
-    const int split1 = sh.split[1], quads = (p.hidden + 3) / 4;
-    for (int at = blockIdx.x * kMoeThreads + threadIdx.x; at < p.tokens * quads; at += gridDim.x * kMoeThreads) {
-        const int t = at / quads, c = (at - t * quads) * 4;      // (the rows of the sums are whole 32s long)
+    // a warp takes 32 channels of a token: 8 lanes 4 each, of every fourth addend; neighbouring lines are in different CTAs
+    const int split1 = sh.split[1], lines = (p.hidden + 31) / 32, addends = p.top * split1;
+    for (int line = warp * gridDim.x + blockIdx.x; line < p.tokens * lines; line += (kMoeThreads / 32) * gridDim.x) {
+        const int t = line / lines, c = (line - t * lines) * 32 + (lane & 7) * 4;      // (the rows of the sums are whole 32s long)
+        const float* rows = p.yp + static_cast<size_t>(t) * p.top * p.split * p.y_pitch + c;
         float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int i0 = 0; i0 < p.top; i0 += 4) {                   // four choices' loads in flight
+#pragma unroll 1
+        for (int a0 = lane >> 3; a0 < addends; a0 += 16) {        // four addends' loads in flight
             float4 y[4];
             float weight[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int row = t * p.top + min(i0 + i, p.top - 1);
-                y[i] = __ldcg(reinterpret_cast<const float4*>(p.yp + static_cast<size_t>(row) * p.split * p.y_pitch + c));
-                weight[i] = __ldcg(p.weights + row);
+                const int a = min(a0 + 4 * i, addends - 1), choice = a / split1, s = a - choice * split1;
+                y[i] = __ldcg(reinterpret_cast<const float4*>(rows + static_cast<size_t>(choice * p.split + s) * p.y_pitch));
+                weight[i] = __ldcg(p.weights + t * p.top + choice);
             }
-            for (int s = 1; s < split1; ++s)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int row = t * p.top + min(i0 + i, p.top - 1);
-                    const float4 more = __ldcg(reinterpret_cast<const float4*>(p.yp + (static_cast<size_t>(row) * p.split + s) * p.y_pitch + c));
-                    y[i].x += more.x; y[i].y += more.y; y[i].z += more.z; y[i].w += more.w;
-                }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                if (i0 + i >= p.top) break;
+                if (a0 + 4 * i >= addends) break;
                 sum.x = fmaf(weight[i], y[i].x, sum.x);
                 sum.y = fmaf(weight[i], y[i].y, sum.y);
                 sum.z = fmaf(weight[i], y[i].z, sum.z);
                 sum.w = fmaf(weight[i], y[i].w, sum.w);
             }
         }
+#pragma unroll
+        for (int o = 8; o < 32; o <<= 1) {
+            sum.x += __shfl_xor_sync(0xFFFFFFFFu, sum.x, o);
+            sum.y += __shfl_xor_sync(0xFFFFFFFFu, sum.y, o);
+            sum.z += __shfl_xor_sync(0xFFFFFFFFu, sum.z, o);
+            sum.w += __shfl_xor_sync(0xFFFFFFFFu, sum.w, o);
+        }
+        if (lane >= 8) continue;
         const uint32_t lo = float_to_pair<BF16>(sum.x, sum.y), hi = float_to_pair<BF16>(sum.z, sum.w);
         uint16_t* dst = p.y + t * p.ldy + c;
-        dst[0] = static_cast<uint16_t>(lo);
+        if (c < p.hidden) dst[0] = static_cast<uint16_t>(lo);
         if (c + 1 < p.hidden) dst[1] = static_cast<uint16_t>(lo >> 16);
         if (c + 2 < p.hidden) dst[2] = static_cast<uint16_t>(hi);
         if (c + 3 < p.hidden) dst[3] = static_cast<uint16_t>(hi >> 16);
