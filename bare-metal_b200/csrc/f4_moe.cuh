@@ -8,10 +8,12 @@
 // The products run on tcgen05.mma.kind::mxf4nvf4, which takes the weights as they are stored; nothing is done per weight outside
 // the tensor core.  (Converting them to fp16 in registers for mma.sync took 2.2 instructions a weight and reached
 // 1.9 TB/s; the conversion instruction alone runs at 16 weights a clock and SM, a third of what HBM delivers.)  It wants
-// the activations in 4 bits too, so each is a SUM of 6 block-scaled E2M1 numbers: the nearest one, the nearest one to what is
-// left, and so on.  With E4M3 scales what is left shrinks by at least 5.6 a step, with powers of two by 8 after the first: 2^-15 of
-// the block's largest at the end, less than fp16's own rounding of it (2^-12).  The six are six columns of the MMA and cost
-// nothing: an MMA takes as long with 8 columns as with 100.  fp32 sums; a token's six columns are added at the end.
+// the activations in 4 bits too, so each is written with six digits of base 8 under its block's scale,
+//     x = s * sum over i < 6 of 8^-i * d_i / 2,   d_i from -4 to 3: all of them E2M1 numbers when halved,
+// which leaves 2^-17 s < 2^-16.7 of the block's largest, far less than fp16's own rounding of it (2^-12).  The six digits are six
+// columns of the MMA and cost nothing: an MMA takes as long with 8 columns as with 100.  All six have the block's scale;
+// the powers of 8 are applied to the columns' fp32 sums when they are added.  (Six E2M1 numbers by repeated rounding of what is left
+// are as exact and took three times the instructions.)
 //
 // Kernel 1, moe_router_kernel: a cluster of 8 CTAs per group of at most 4 tokens.  128 warps share the experts, each
 // token's logits meet in the shared memory of one CTA, whose first warp selects, while the other warps cut x into its six parts.
@@ -38,12 +40,12 @@ constexpr int kMoeMaxTokens = 64;
 constexpr int kMoeMaxExperts = 256;
 constexpr int kMoeMaxTop = 16;
 constexpr int kMoeMaxDim = 16384;
-constexpr int kMoeParts = 6;                                    // E2M1 numbers an activation is the sum of
+constexpr int kMoeParts = 6;                                    // digits of an activation
 constexpr int kMoeMaxSplit = 4;                                 // pieces of K of a unit at most
 constexpr int kMoeMaxRuns = 112;
 
-// Activations cut up: per token and 256 of K 1 KiB, 8 rows (6 used) of 128 bytes in the 128-byte swizzle of an MMA operand, and the
-// scales, per token and tile of 4 blocks 8 rows (6 used) of 4 bytes.
+// Activations cut up: per token and 256 of K 1 KiB, 8 rows (the 6 digits) of 128 bytes in the 128-byte swizzle of an MMA operand, and the
+// scales, per token and tile of 4 blocks 8 rows (the same for 6) of 4 bytes.
 __host__ __device__ constexpr int moe_k_blocks(int k) { return (k + kF4BK - 1) / kF4BK; }
 __host__ __device__ constexpr int moe_value_bytes(int k) { return moe_k_blocks(k) * 1024; }
 __host__ __device__ constexpr int moe_scale_bytes(int k, int fmt) { return moe_k_blocks(k) * f4_stage_tiles(fmt) * 32; }
@@ -92,68 +94,65 @@ __device__ __forceinline__ uint4 moe_piece(const uint16_t* row, int v, int k, bo
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// FMT_E4M3: the power of two that puts a row with largest |v| = top (fp32 bits) where the quantiser puts it, and its inverse
+// FMT_E4M3: the power of two 2^e that puts a row's largest |v| (fp32 bits) in [2^8, 2^9), where 0.625 times it is a scale, as v / 2^e
 template <int FMT>
 __device__ __forceinline__ void moe_row_factor(uint32_t top_bits, float& factor, float& inv) {
     factor = inv = 1.f;
     if (FMT == FMT_E8M0 || top_bits == 0 || top_bits >= 0x7F800000u) return;
-    const int lg = static_cast<int>(top_bits >> 23), e = lg > 11 ? lg - 10 : 1;
+    const int lg = static_cast<int>(top_bits >> 23), e = lg > 9 ? lg - 8 : 1;
     factor = __uint_as_float(static_cast<uint32_t>(e) << 23);
     inv = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
 }
 
-// Eight activations (piece v of a row, two or four neighbouring lanes share a block) cut into E2M1 numbers with scales.  `values`,
-// `scales`: the token's own places, in shared or global memory.  Whole warps; `live` lanes store.
+// Eight activations (piece v of a row, two or four neighbouring lanes share a block) as digits and scales.  `values`, `scales`: the
+// token's own places, in shared or global memory.  Whole warps.
+//   The scale is at least |largest| / 1.7067: six digits reach 1.714.  A number times 2^16 / s, rounded to an integer m, plus 4 in every
+// digit, are the 18 low bits of the sum with 1.5 * 2^23: one FMA, and digit + 4 are three of its bits.
 template <int FMT>
-__device__ __forceinline__ void moe_cut(float (&r)[8], int v, bool live, uint8_t* values, uint8_t* scales) {
+__device__ __forceinline__ void moe_cut(const float (&x)[8], int v, uint8_t* values, uint8_t* scales) {
     constexpr int SHARE = f4_block(FMT) / 8;
-    const int block = v / SHARE;
-    uint8_t* row = values + (v >> 5) * 1024 + (v & 3) * 4;
-    uint8_t* scale = scales + (block >> 2) * 32 + (block & 3);
-    const int chunk = (v & 31) >> 2;
     float odd = 0.f;                                              // a NaN where one of the block's numbers is none
 #pragma unroll
-    for (int j = 0; j < 8; ++j) odd = fmaf(r[j], 0.f, odd);
+    for (int j = 0; j < 8; ++j) odd = fmaf(x[j], 0.f, odd);
+    float top = fmaxf(fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))),
+                      fmaxf(fmaxf(fabsf(x[4]), fabsf(x[5])), fmaxf(fabsf(x[6]), fabsf(x[7]))));
 #pragma unroll
-    for (int o = 1; o < SHARE; o <<= 1) odd += __shfl_xor_sync(0xFFFFFFFFu, odd, o);
-#pragma unroll 1                                                  // (code that runs once waits for its own fetch)
+    for (int o = 1; o < SHARE; o <<= 1) {
+        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+        odd += __shfl_xor_sync(0xFFFFFFFFu, odd, o);
+    }
+    uint32_t byte;
+    float inv;                                                    // 2^16 / s
+    if constexpr (FMT == FMT_E4M3) {
+        // to the nearest, off by a 16th at most; half a step more where steps are even (below 2^-6), so never below there
+        byte = __nv_cvt_float_to_fp8(fmaf(top, 0.625f, 0x1p-10f), __NV_SATFINITE, __NV_E4M3);
+        inv = byte != 0 ? __fdividef(65536.f, e4m3_value(byte)) : 0.f;
+    } else {
+        // the smallest power of two that holds the largest below 1.7 (2^-110 at least: what is smaller is nothing in fp32 sums)
+        byte = max(min((__float_as_uint(top * 0.58823530f) + 0x007FFFFFu) >> 23, 253u), 17u);
+        inv = __uint_as_float((254u + 16u - byte) << 23);
+    }
+    uint32_t t[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) t[j] = __float_as_uint(fmaf(x[j], inv, 12582912.f + 149796.f));
+    const int block = v / SHARE, chunk = (v & 31) >> 2;
+    uint8_t* row = values + (v >> 5) * 1024 + (v & 3) * 4;
+    uint8_t* scale = scales + (block >> 2) * 32 + (block & 3);
+    if (odd != 0.f) byte = FMT == FMT_E4M3 ? 127u : 255u;
+#pragma unroll
     for (int i = 0; i < kMoeParts; ++i) {
-        float top = fmaxf(fmaxf(fmaxf(fabsf(r[0]), fabsf(r[1])), fmaxf(fabsf(r[2]), fabsf(r[3]))),
-                          fmaxf(fmaxf(fabsf(r[4]), fabsf(r[5])), fmaxf(fabsf(r[6]), fabsf(r[7]))));
+        constexpr int kTopDigit = 3 * (kMoeParts - 1);
+        uint32_t u = 0;                                           // digits + 4, a nibble each
 #pragma unroll
-        for (int o = 1; o < SHARE; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-        const float sixth = top * 0.16666667f;
-        uint32_t byte;
-        float s, inv;
-        if constexpr (FMT == FMT_E4M3) {
-            byte = __nv_cvt_float_to_fp8(sixth, __NV_SATFINITE, __NV_E4M3);
-            s = e4m3_value(byte);
-            inv = s > 0.f ? __fdividef(1.f, s) : 0.f;
-        } else {
-            // the smallest power of two that holds the largest below 6 (or a rounding above it)
-            const uint32_t b = __float_as_uint(sixth);
-            byte = min((b + 0x007FFFFFu) >> 23, 253u);
-            s = e8m0_value(byte);
-            inv = __uint_as_float((254u - byte) << 23);
+        for (int j = 0; j < 8; ++j) {
+            const int shift = 4 * j - (kTopDigit - 3 * i);
+            u |= (shift >= 0 ? t[j] << (shift & 31) : t[j] >> (-shift & 31)) & (7u << (4 * j));
         }
-        float y[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] = r[j] * inv;
-        const uint32_t codes = e2m1x8(y);
-        if (live) {
-            *reinterpret_cast<uint32_t*>(row + i * 128 + ((chunk ^ i) << 4)) = codes;
-            if (v % SHARE == 0) scale[i * 4] = static_cast<uint8_t>(odd == 0.f ? byte : FMT == FMT_E4M3 ? 127u : 255u);
-        }
-        uint32_t h[4];
-        e2m1x8_to_small_half(codes, h);
-        constexpr int kOrder[4] = {1, 3, 0, 2};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const __half2 whole = __hmul2(*reinterpret_cast<const __half2*>(&h[j]), __float2half2_rn(16384.f));
-            const float2 f = __half22float2(whole);
-            r[kOrder[j]] = fmaf(-f.x, s, r[kOrder[j]]);
-            r[kOrder[j] + 4] = fmaf(-f.y, s, r[kOrder[j] + 4]);
-        }
+        // 4 + d -> the code of d / 2: d itself, or 8 | -d
+        const uint32_t neg = (~u >> 2) & 0x11111111u;
+        const uint32_t codes = (((u & 0x33333333u) ^ (neg * 3u)) + neg) | (neg << 3);
+        *reinterpret_cast<uint32_t*>(row + i * 128 + ((chunk ^ i) << 4)) = codes;
+        if (v % SHARE == 0) scale[i * 4] = static_cast<uint8_t>(byte);
     }
 }
 
@@ -267,7 +266,7 @@ moe_router_kernel(const MoeParams p) {
                 f[2 * j] = two.x * inv;
                 f[2 * j + 1] = two.y * inv;
             }
-            moe_cut<FMT>(f, v, true, values, scales);
+            moe_cut<FMT>(f, v, values, scales);
         }
         return;
     }
@@ -709,7 +708,7 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_con
                         up[0] += u0.x; up[1] += u0.y; up[2] += u0.z; up[3] += u0.w; up[4] += u1.x; up[5] += u1.y; up[6] += u1.z; up[7] += u1.w;
                     }
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) h[i] = v * 8 + i < k ? __fdividef(h[i], 1.f + expf(-h[i])) * up[i] : 0.f;      // (nobody wrote what is behind)
+                    for (int i = 0; i < 8; ++i) h[i] = v * 8 + i < k ? __fdividef(h[i], 1.f + __expf(-h[i])) * up[i] : 0.f;      // (nobody wrote what is behind)
                 };
                 if constexpr (FMT == FMT_E4M3) {                  // the rows' factors first; the numbers wait in the tile
 #pragma unroll 1
@@ -751,7 +750,7 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_con
                     } else {
                         hidden(j, kb, h);
                     }
-                    moe_cut<FMT>(h, kb * 32 + lane, true, tile + j * value_bytes, tile_scales + j * scale_pitch);
+                    moe_cut<FMT>(h, kb * 32 + lane, tile + j * value_bytes, tile_scales + j * scale_pitch);
                 }
                 fence_proxy_async_smem();                         // visible to the tensor core
                 __syncwarp();
@@ -829,7 +828,7 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_con
                         tmem_ld_wait();
                         float sum = __uint_as_float(v[kMoeParts - 1]);        // the smallest first
 #pragma unroll
-                        for (int i = kMoeParts - 2; i >= 0; --i) sum += __uint_as_float(v[i]);
+                        for (int i = kMoeParts - 2; i >= 0; --i) sum = fmaf(sum, 0.125f, __uint_as_float(v[i]));
                         if (in) __stcg(out + slot_row[j] * step, sum * factor * slot_scale[j]);
                     }
                     tc_fence_before_sync();

@@ -36,20 +36,19 @@ class Layer:
         return logits, order, p / (p if self.norm else z).sum(1, keepdims=True)
 
     def left(self, v, dv=0.0):
-        """What six E2M1 numbers may leave of rows of activations (known up to dv)."""
+        """What the digits may leave of rows of activations (known up to dv)."""
         a = np.abs(v) + dv
         n = f4.BLOCK[self.fmt]
         top = np.pad(a, ((0, 0), (0, -a.shape[1] % n))).reshape(a.shape[0], -1, n).max(-1).repeat(n, 1)[:, :a.shape[1]]
-        return 2.0 ** -14.9 * top + (2.0 ** -17.4 * a.max(1, keepdims=True) if self.fmt == ig.BM_F4_E4M3 else 0.0)
+        return 2.0 ** -16.7 * top + 2.0 ** -34 * a.max(1, keepdims=True)
 
     def check(self, y, ids, weights):
         """Errors: an fp32 sum over K is off by at most 2^-23 of the sum of sizes for each of K / 16 + 32 additions (truncated);
-        SiLU moves by at most 1.1 times what its argument does, its evaluation is off by 8 units of 2^-24.  Activations and hidden
-        activations are sums of six E2M1 numbers with block scales.  With scale s = E4M3(amax / 6) the nearest E2M1 number leaves
-        at most s <= 1.0625 amax / 6, a part in 5.6: 5.6^-6 < 2^-14.9 of the block's largest after six; scales below 2^-10 of
-        the row's unit are zero and leave 6 * 2^-10 of it, where the row's largest is 2^10 units or more: 2^-17.4.  With
-        powers of two, amax / s in (3, 6], the first leaves s <= amax / 3 and every further one an eighth: 2^-16.5.  (A block is at most 32
-        long.)  Then the sum over the choices, and the rounding to the output type."""
+        SiLU moves by at most 1.1 times what its argument g does; its evaluation is off by 8 + |g| units of 2^-24 (the exponent g
+        log2(e) is rounded).  Activations and hidden activations are written with six digits of base 8: off by at most half a
+        unit, s / 2 * 8^-5 / 2 = 2^-17 s, and s is at most 2 / 1.7 of the block's largest (a power of two), or 1.0625 / 1.6 of it (E4M3;
+        at least 2^-9 of a unit of which the row's largest has 2^8 or more): 2^-16.7 of the block's, 2^-34 of the row's.  (A
+        block is at most 32 long.)  Then the sum over the choices, and the rounding to the output type."""
         logits, order, p = self.select()
         ranked = -np.sort(-logits, 1)
         if self.top < self.E:
@@ -69,7 +68,7 @@ class Layer:
                 g, u = gu[:self.I], gu[self.I:]
                 s = g / (1 + np.exp(-g))
                 h = s * u
-                dh = 1.1 * du[:self.I] * (np.abs(u) + du[self.I:]) + np.abs(s) * du[self.I:] + np.abs(h) * 2.0 ** -21
+                dh = 1.1 * du[:self.I] * (np.abs(u) + du[self.I:]) + np.abs(s) * du[self.I:] + np.abs(h) * (8 + np.abs(g)) * 2.0 ** -24
                 dh = dh + self.left(h[None], dh[None])[0]
                 y1, d1 = b @ h, np.abs(b) @ dh + u2 * (np.abs(b) @ np.abs(h))
                 want[t] += p[t, k] * y1
