@@ -355,13 +355,16 @@ moe_router_kernel(const MoeParams p) {
 #endif
 constexpr int kMoeBuilderWarps = BM_MOE_BUILDERS;
 constexpr int kMoeBuilders = 32 * kMoeBuilderWarps;             // the last warps
-constexpr int kMoeThreads = 10 * 32 + kMoeBuilders;             // TMA producer, MMA issuer, 4 scale warps, 4 epilogue warps, builders
-constexpr int kMoeStages = 4;
+constexpr int kMoeFirstBuilder = 11;
+constexpr int kMoeThreads = kMoeFirstBuilder * 32 + kMoeBuilders;   // values producer, MMA issuer, 4 scale warps, 4 epilogue warps, scales producer, builders
+constexpr int kMoeStages = 4;                                   // weight values, 256 of K
+constexpr int kMoeScaleStages = 4;                              // their scales, on their way ...
+constexpr int kMoeSfBufs = 4;                                   // ... to tensor memory
 constexpr int kMoeTileTokens = 16;                              // tokens of a pass at most: 128 MMA columns
 constexpr int kMoeTileBytes = 128 * 1024;                       // activations of a pass: 8 tokens of 4096, 16 of 2048
 constexpr int kMoeTileScales = 17 * 1024;
 constexpr int kMoeStageValues = 128 * 128, kMoeStageScales = 128 * 16;
-constexpr int kMoeAccStride = 128, kMoeSfBase = 256;            // tensor memory: two accumulators, two sets of scales (32 columns each)
+constexpr int kMoeAccStride = 128, kMoeSfBase = 256;            // tensor memory: two accumulators, four sets of scales (32 columns each)
 
 // Tiles of activations: one, or two halves where a half holds 8 tokens, so that the next is made while one is multiplied.
 __host__ __device__ constexpr int moe_tiles(int k) { return 8 * moe_value_bytes(k) <= kMoeTileBytes / 2 ? 2 : 1; }
@@ -389,10 +392,11 @@ struct MoeShared {
     uint32_t slot_top[2][kMoeTileTokens];        // per run (mod 2): largest hidden activation, fp32 bits
     int abort_flag;
     uint32_t tmem_slot;
-    unsigned long long full[kMoeStages], empty[kMoeStages], sf_full[2], sf_empty[2], acc_full[2], acc_empty[2], tile_full[2][2], tile_empty[2][2], drain;
+    unsigned long long full[kMoeStages], empty[kMoeStages], scale_full[kMoeScaleStages], scale_empty[kMoeScaleStages], sf_full[kMoeSfBufs], sf_empty[kMoeSfBufs];
+    unsigned long long acc_full[2], acc_empty[2], tile_full[2][2], tile_empty[2][2], drain;
 };
 constexpr int kMoeStageScaleOffset = kMoeStages * kMoeStageValues;
-constexpr int kMoeTileOffset = kMoeStageScaleOffset + kMoeStages * kMoeStageScales;
+constexpr int kMoeTileOffset = (kMoeStageScaleOffset + kMoeScaleStages * kMoeStageScales + 1023) / 1024 * 1024;
 constexpr int kMoeTileScaleOffset = kMoeTileOffset + kMoeTileBytes;
 constexpr int kMoeSharedOffset = kMoeTileScaleOffset + kMoeTileScales;
 constexpr int kMoeSmemBytes = kMoeSharedOffset + static_cast<int>(sizeof(MoeShared)) + 1024;
@@ -443,9 +447,15 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_con
             mbar_init(bar_of(sh.full[i]), 1);
             mbar_init(bar_of(sh.empty[i]), 1);
         }
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < kMoeScaleStages; ++i) {
+            mbar_init(bar_of(sh.scale_full[i]), 1);
+            mbar_init(bar_of(sh.scale_empty[i]), 4);
+        }
+        for (int i = 0; i < kMoeSfBufs; ++i) {
             mbar_init(bar_of(sh.sf_full[i]), 4);
             mbar_init(bar_of(sh.sf_empty[i]), 1);
+        }
+        for (int i = 0; i < 2; ++i) {
             mbar_init(bar_of(sh.acc_full[i]), 1);
             mbar_init(bar_of(sh.acc_empty[i]), 4);
         }
@@ -545,28 +555,36 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_con
     };
 
     // Every role goes through the CTA's runs, their elements and these elements' stages in the same order.
-    if (warp == 0) {
-        // ------------------------------------------------------------------ producer: weights and their scales
+    if (warp == 0 || warp == 10) {
+        // ------------------------------------------------------------------ producers: the weights' values, and their scales.  The scales run
+        // further ahead: they are in tensor memory when the values arrive, and a stage of these is held for its MMAs only.
+        const bool is_scales = warp == 10;
+        const uint32_t stages = is_scales ? kMoeScaleStages : kMoeStages;
         uint32_t stage = 0, phase = 0;
         bool ok = true;
         for (int it = 0; it < runs && ok; ++it) {
             const int ph = it >= count0, split = sh.split[ph];
             const MoeRun r = sh.runs[ph][ph ? it - count0 : it];
-            const CUtensorMap* values = ph ? &map_w2 : &map_w13;
-            const CUtensorMap* scales = ph ? &map_s2 : &map_s13;
+            const CUtensorMap* map = is_scales ? (ph ? &map_s2 : &map_s13) : (ph ? &map_w2 : &map_w13);
             for (int el = r.first; el < r.last && ok; ++el) {
                 const int unit = el / split, piece = el - unit * split;
                 const int kb1 = items[ph] * (piece + 1) / split, row = unit * (ph ? 128 : 64), outer = ph ? r.expert : 2 * r.expert;
                 for (int kb = items[ph] * piece / split; kb < kb1; ++kb) {
-                    if (!warp_bounded_wait(bar_of(sh.empty[stage]), phase ^ 1u, abort_flag, p.status, DEV_TIMEOUT_PRODUCER_EMPTY)) { ok = false; break; }
+                    if (!warp_bounded_wait(is_scales ? bar_of(sh.scale_empty[stage]) : bar_of(sh.empty[stage]), phase ^ 1u, abort_flag, p.status,
+                                           DEV_TIMEOUT_PRODUCER_EMPTY)) { ok = false; break; }
                     if (elect_one()) {
-                        const uint32_t bar = bar_of(sh.full[stage]);
-                        mbar_expect_tx(bar, kMoeStageValues + kMoeStageScales);
-                        tma_load_3d(smem_base + stage * kMoeStageValues, values, bar, kb * 128, row, outer);
-                        tma_load_3d(smem_base + kMoeStageScaleOffset + stage * kMoeStageScales, scales, bar, (FMT == FMT_E4M3 ? kb : kb >> 1) * 16, row, outer);
+                        if (is_scales) {
+                            const uint32_t bar = bar_of(sh.scale_full[stage]);
+                            mbar_expect_tx(bar, kMoeStageScales);
+                            tma_load_3d(smem_base + kMoeStageScaleOffset + stage * kMoeStageScales, map, bar, (FMT == FMT_E4M3 ? kb : kb >> 1) * 16, row, outer);
+                        } else {
+                            const uint32_t bar = bar_of(sh.full[stage]);
+                            mbar_expect_tx(bar, kMoeStageValues);
+                            tma_load_3d(smem_base + stage * kMoeStageValues, map, bar, kb * 128, row, outer);
+                        }
                     }
                     __syncwarp();
-                    if (++stage == kMoeStages) { stage = 0; phase ^= 1u; }
+                    if (++stage == stages) { stage = 0; phase ^= 1u; }
                 }
             }
         }
@@ -586,8 +604,8 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_con
                 const int kb0 = items[ph] * piece / split, kb1 = items[ph] * (piece + 1) / split;
                 if (!warp_bounded_wait(bar_of(sh.acc_empty[acc]), acc_phase ^ 1u, abort_flag, p.status, DEV_TIMEOUT_MMA_ACC_EMPTY)) { ok = false; break; }
                 for (int kb = kb0; kb < kb1; ++kb) {
-                    if (!warp_bounded_wait(bar_of(sh.full[stage]), phase, abort_flag, p.status, DEV_TIMEOUT_MMA_FULL) ||
-                        !warp_bounded_wait(bar_of(sh.sf_full[buf]), buf_phase, abort_flag, p.status, DEV_TIMEOUT_MMA_FULL)) { ok = false; break; }
+                    if (!warp_bounded_wait(bar_of(sh.sf_full[buf]), buf_phase, abort_flag, p.status, DEV_TIMEOUT_MMA_FULL) ||
+                        !warp_bounded_wait(bar_of(sh.full[stage]), phase, abort_flag, p.status, DEV_TIMEOUT_MMA_FULL)) { ok = false; break; }
                     tc_fence_after_sync();
                     if (elect_one()) {
                         const uint32_t d = tmem_base + acc * kMoeAccStride, sfa = tmem_base + kMoeSfBase + buf * 32, sfb = sfa + 16;
@@ -605,8 +623,7 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_con
                     }
                     __syncwarp();
                     if (++stage == kMoeStages) { stage = 0; phase ^= 1u; }
-                    buf ^= 1u;
-                    if (buf == 0) buf_phase ^= 1u;
+                    if (++buf == kMoeSfBufs) { buf = 0; buf_phase ^= 1u; }
                 }
                 if (!ok) break;
                 if (elect_one()) tc_commit(bar_of(sh.acc_full[acc]));
@@ -626,7 +643,7 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_con
         }
     } else {
         // ------------------------------------------------------------------ scale warps, epilogue warps and builders
-        const int quarter = warp & 3, tid = static_cast<int>(threadIdx.x) - 320;
+        const int quarter = warp & 3, tid = static_cast<int>(threadIdx.x) - 32 * kMoeFirstBuilder;
         const bool scales_role = warp < 6, epilogue_role = warp >= 6 && warp < 10;
         uint32_t stage = 0, phase = 0, buf = 0, buf_phase = 0, acc = 0, acc_phase = 0;
         bool ok = true;                                           // a builder that gave up still meets the others at their barriers
@@ -646,7 +663,7 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_con
                 };
                 wait_empty(ph, tile_at, (tile_use & 1) ^ 1);
                 if (ph == 0) {
-                    if (warp == 10 && ok) {                       // copies what the router kernel has cut
+                    if (warp == kMoeFirstBuilder && ok) {                       // copies what the router kernel has cut
                         const uint32_t bar = bar_of(sh.tile_full[0][tile_at]);
                         const int scale_bytes = moe_scale_bytes(k, FMT);
                         int t = 0;
@@ -692,30 +709,40 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_con
                 builders_sync();
                 // a warp takes 256 activations of a token at a time: 1 KiB of the tile, in fp32 as well as cut up
                 const int split0 = sh.split[0];
-                auto hidden = [&](int j, int kb, float (&h)[8]) {
-                    const int v = kb * 32 + lane;
-                    const float* src = p.gu + static_cast<size_t>(slot_row[j]) * p.split * p.gu_pitch + v * 8;
-                    float up[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) h[i] = up[i] = 0.f;
-                    if (v * 8 >= k) return;
+                const int tasks = n * items[1];
+                struct Sums { float4 g0, g1, u0, u1; };
+                auto source = [&](int at) {
+                    const int j = at / items[1], v = (at - j * items[1]) * 32 + lane;
+                    return p.gu + static_cast<size_t>(slot_row[j]) * p.split * p.gu_pitch + v * 8;
+                };
+                auto load = [&](const float* src) {
+                    const float4* gp = reinterpret_cast<const float4*>(src);
+                    const float4* upp = reinterpret_cast<const float4*>(src + p.gu_pitch / 2);
+                    return Sums{__ldcg(gp), __ldcg(gp + 1), __ldcg(upp), __ldcg(upp + 1)};
+                };
+                Sums next{};                                      // the task after the one at hand is on its way
+                if (warp - kMoeFirstBuilder < tasks) next = load(source(warp - kMoeFirstBuilder));
+                auto hidden = [&](int at, float (&h)[8]) {
+                    const Sums c = next;
+                    if (at + kMoeBuilderWarps < tasks) next = load(source(at + kMoeBuilderWarps));
+                    float g[8] = {c.g0.x, c.g0.y, c.g0.z, c.g0.w, c.g1.x, c.g1.y, c.g1.z, c.g1.w};
+                    float up[8] = {c.u0.x, c.u0.y, c.u0.z, c.u0.w, c.u1.x, c.u1.y, c.u1.z, c.u1.w};
 #pragma unroll 1
-                    for (int s = 0; s < split0; ++s, src += p.gu_pitch) {
-                        const float4* gp = reinterpret_cast<const float4*>(src);
-                        const float4* upp = reinterpret_cast<const float4*>(src + p.gu_pitch / 2);
-                        const float4 g0 = __ldcg(gp), g1 = __ldcg(gp + 1), u0 = __ldcg(upp), u1 = __ldcg(upp + 1);
-                        h[0] += g0.x; h[1] += g0.y; h[2] += g0.z; h[3] += g0.w; h[4] += g1.x; h[5] += g1.y; h[6] += g1.z; h[7] += g1.w;
-                        up[0] += u0.x; up[1] += u0.y; up[2] += u0.z; up[3] += u0.w; up[4] += u1.x; up[5] += u1.y; up[6] += u1.z; up[7] += u1.w;
+                    for (int s = 1; s < split0; ++s) {
+                        const Sums m = load(source(at) + static_cast<size_t>(s) * p.gu_pitch);
+                        g[0] += m.g0.x; g[1] += m.g0.y; g[2] += m.g0.z; g[3] += m.g0.w; g[4] += m.g1.x; g[5] += m.g1.y; g[6] += m.g1.z; g[7] += m.g1.w;
+                        up[0] += m.u0.x; up[1] += m.u0.y; up[2] += m.u0.z; up[3] += m.u0.w; up[4] += m.u1.x; up[5] += m.u1.y; up[6] += m.u1.z; up[7] += m.u1.w;
                     }
+                    const int k0 = ((at % items[1]) * 32 + lane) * 8;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) h[i] = v * 8 + i < k ? __fdividef(h[i], 1.f + __expf(-h[i])) * up[i] : 0.f;      // (nobody wrote what is behind)
+                    for (int i = 0; i < 8; ++i) h[i] = k0 + i < k ? __fdividef(g[i], 1.f + __expf(-g[i])) * up[i] : 0.f;      // (nobody wrote what is behind)
                 };
                 if constexpr (FMT == FMT_E4M3) {                  // the rows' factors first; the numbers wait in the tile
 #pragma unroll 1
-                    for (int at = warp - 10; at < n * items[1]; at += kMoeBuilderWarps) {
+                    for (int at = warp - kMoeFirstBuilder; at < tasks; at += kMoeBuilderWarps) {
                         const int j = at / items[1], kb = at - j * items[1];
                         float h[8];
-                        hidden(j, kb, h);
+                        hidden(at, h);
                         uint32_t top = 0;
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
@@ -736,7 +763,7 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_con
                     slot_scale[tid] = factor;
                 }
 #pragma unroll 1
-                for (int at = warp - 10; at < n * items[1]; at += kMoeBuilderWarps) {
+                for (int at = warp - kMoeFirstBuilder; at < tasks; at += kMoeBuilderWarps) {
                     const int j = at / items[1], kb = at - j * items[1];
                     float h[8];
                     if constexpr (FMT == FMT_E4M3) {
@@ -748,7 +775,7 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_con
                         h[4] = hi.x * inv; h[5] = hi.y * inv; h[6] = hi.z * inv; h[7] = hi.w * inv;
                         __syncwarp();                             // all lanes have theirs: the cut numbers take the place
                     } else {
-                        hidden(j, kb, h);
+                        hidden(at, h);
                     }
                     moe_cut<FMT>(h, kb * 32 + lane, tile + j * value_bytes, tile_scales + j * scale_pitch);
                 }
@@ -769,7 +796,7 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_con
                     const int unit = el / split, piece = el - unit * split;
                     const int kb1 = items[ph] * (piece + 1) / split;
                     for (int kb = items[ph] * piece / split; kb < kb1; ++kb) {
-                        if (!warp_bounded_wait(bar_of(sh.full[stage]), phase, abort_flag, p.status, DEV_TIMEOUT_MMA_FULL)) { ok = false; break; }
+                        if (!warp_bounded_wait(bar_of(sh.scale_full[stage]), phase, abort_flag, p.status, DEV_TIMEOUT_MMA_FULL)) { ok = false; break; }
                         const uint4* rows = reinterpret_cast<const uint4*>(smem_gen + kMoeStageScaleOffset + stage * kMoeStageScales);
                         uint32_t a[16], b[16];
 #pragma unroll
@@ -788,6 +815,8 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_con
                                 b[t * 4 + c] = t < KT && c < groups && c * 4 + token < n
                                                    ? *reinterpret_cast<const uint32_t*>(tile_scales + (c * 4 + token) * scale_pitch + (kb * KT + t) * 32 + part * 4)
                                                    : 0u;
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(bar_of(sh.scale_empty[stage]));
                         if (!warp_bounded_wait(bar_of(sh.sf_empty[buf]), buf_phase ^ 1u, abort_flag, p.status, DEV_TIMEOUT_MMA_ACC_EMPTY)) { ok = false; break; }
                         tc_fence_after_sync();
                         tmem_st_32x16(tmem_base + lanes + kMoeSfBase + buf * 32, a);
@@ -796,9 +825,8 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_con
                         tc_fence_before_sync();
                         __syncwarp();
                         if (lane == 0) mbar_arrive(bar_of(sh.sf_full[buf]));
-                        if (++stage == kMoeStages) { stage = 0; phase ^= 1u; }
-                        buf ^= 1u;
-                        if (buf == 0) buf_phase ^= 1u;
+                        if (++stage == kMoeScaleStages) { stage = 0; phase ^= 1u; }
+                        if (++buf == kMoeSfBufs) { buf = 0; buf_phase ^= 1u; }
                     }
                 }
             } else {
