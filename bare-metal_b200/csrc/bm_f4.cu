@@ -21,6 +21,12 @@ static size_t f4_scale_bytes(int rows, int k, int fmt, int layout) {
     return layout == BM_SCALE_TILED ? static_cast<size_t>(ceil_div(rows, 128)) * f4_tiles_k(k, fmt) * kF4TileBytes
                                     : static_cast<size_t>(rows) * f4_scale_pitch(k, fmt);
 }
+// the widest access, up to 16 bytes, that a matrix with this base and pitch allows at every eighth column
+static int access_bytes(const void* p, size_t pitch) {
+    int n = 16;
+    while ((reinterpret_cast<uintptr_t>(p) | pitch) % n != 0) n /= 2;
+    return n;
+}
 static bool aligned_to(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
 // ---- quantise ---------------------------------------------------------------------------
@@ -45,12 +51,16 @@ static int launch_quantize(const F4QuantParams& p, int sms, cudaStream_t stream)
 }
 
 template <int FMT>
-static int launch_dequantize(const F4DequantParams& p, int type, int sms, cudaStream_t stream) {
-    const long long threads = static_cast<long long>(p.rows) * ceil_div(p.k, 8), blocks = (threads + 255) / 256;
-    const unsigned grid = static_cast<unsigned>(blocks < 64ll * sms ? blocks : 64ll * sms);
-    if (type == TYPE_F16) dequantize_f4_kernel<FMT, TYPE_F16><<<grid, 256, 0, stream>>>(p);
-    else if (type == TYPE_BF16) dequantize_f4_kernel<FMT, TYPE_BF16><<<grid, 256, 0, stream>>>(p);
-    else dequantize_f4_kernel<FMT, TYPE_F32><<<grid, 256, 0, stream>>>(p);
+static int launch_dequantize(const F4DequantParams& p, int type, cudaStream_t stream) {
+    // rows side by side in a CTA where a row is less than 256 pieces
+    int x = 256;
+    while (x > 32 && x / 2 >= ceil_div(p.k, 8)) x /= 2;
+    const dim3 block(x, 256 / x);
+    const int y = ceil_div(p.rows, static_cast<int>(block.y) * kF4DequantRows);
+    const dim3 grid(ceil_div(ceil_div(p.k, 8), x), y < 65535 ? y : 65535);
+    if (type == TYPE_F16) dequantize_f4_kernel<FMT, TYPE_F16><<<grid, block, 0, stream>>>(p);
+    else if (type == TYPE_BF16) dequantize_f4_kernel<FMT, TYPE_BF16><<<grid, block, 0, stream>>>(p);
+    else dequantize_f4_kernel<FMT, TYPE_F32><<<grid, block, 0, stream>>>(p);
     BM_CUDA_TRY(cudaGetLastError());
     return BM_OK;
 }
@@ -266,7 +276,7 @@ int bm_quantize_f4(const void* X, int x_type, uint8_t* Q, uint8_t* S, float* row
         p.pieces = p.scale_pitch * share;
         p.rows_padded = R;
     }
-    p.vec_ok = aligned16(X) && ldx % 8 == 0;
+    p.vec_bytes = access_bytes(X, static_cast<size_t>(ldx) * 2);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (format == BM_F4_E8M0) return x_type == BM_BF16 ? launch_quantize<FMT_E8M0, true>(p, sms, st) : launch_quantize<FMT_E8M0, false>(p, sms, st);
     return x_type == BM_BF16 ? launch_quantize<FMT_E4M3, true>(p, sms, st) : launch_quantize<FMT_E4M3, false>(p, sms, st);
@@ -282,8 +292,6 @@ int bm_dequantize_f4(const uint8_t* Q, const uint8_t* S, const float* row_scale,
     const size_t elem = out_type == BM_F32 ? 4 : 2;
     if (!aligned16(Q) || !aligned16(S) || !aligned_to(out, elem) || !aligned_to(row_scale, 4))
         return fail_msg(BM_ERR_ALIGN, "Q and S must be 16-byte aligned, the output and row_scale to their elements");
-    int sms = 0;
-    if (int rc = sm_count(&sms)) return rc;
     F4DequantParams p{};
     p.q = Q;
     p.s = S;
@@ -295,9 +303,9 @@ int bm_dequantize_f4(const uint8_t* Q, const uint8_t* S, const float* row_scale,
     p.k_padded = 2 * f4_row_bytes(K);
     if (scale_layout == BM_SCALE_TILED) p.tiles_k = f4_tiles_k(K, format);
     else p.scale_pitch = f4_scale_pitch(K, format);
-    p.vec_ok = aligned16(out) && (static_cast<size_t>(ldo) * elem) % 16 == 0;
+    p.vec_bytes = access_bytes(out, static_cast<size_t>(ldo) * elem);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    return format == BM_F4_E8M0 ? launch_dequantize<FMT_E8M0>(p, out_type, sms, st) : launch_dequantize<FMT_E4M3>(p, out_type, sms, st);
+    return format == BM_F4_E8M0 ? launch_dequantize<FMT_E8M0>(p, out_type, st) : launch_dequantize<FMT_E4M3>(p, out_type, st);
 }
 
 int bm_f4_gemm(const uint8_t* A, const uint8_t* SA, const float* ra, const uint8_t* W, const uint8_t* SW, const float* rw, void* D,

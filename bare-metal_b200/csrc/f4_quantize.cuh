@@ -8,11 +8,13 @@
 // an infinity or a NaN gets the scale NaN and the values 0, so it shows in every product.
 //
 // Everything is exactly determined: x * 2^n is exact, x has at most 11 bits and s at most 4, so x / s is either a tie
-// (a multiple of 1/4) or off every tie by more than 2^-13.  x * (1 / s) in fp32 is within 2^-21 of x / s; adding and
+// (a multiple of 1/4) or off every tie by more than 2^-13.  x * (1 / s) in fp32 is within 2^-20 of x / s; adding and
 // subtracting 768 rounds it to a multiple of 2^-14, which puts ties back on the tie and moves nothing across one.
 //
 // 2 bytes in and 1/2 + 1/16 (1/32) out per element.  A group of threads per row holds it in registers (16-byte pieces
-// of 8 numbers; two or four neighbouring threads share a block), so the row's maximum costs no second read.
+// of 8 numbers; two or four neighbouring threads share a block), so the row's maximum costs no second read.  What bounds it with
+// many rows is instructions as much as bytes, so an element gets one conversion, one FMA and one subtraction before the packing
+// conversion, and a piece's maximum is taken once.
 #pragma once
 #include "f4_format.cuh"
 
@@ -31,35 +33,45 @@ struct F4QuantParams {
     int pieces;                  // pieces of 8 numbers that the stored scales of a row cover
     int tiles_k;                 // tiled scales: tiles along a row; 0: scales in rows
     int scale_pitch;             // scales in rows: bytes of a row
-    int vec_ok;                  // X allows 16-byte loads
+    int vec_bytes;               // X allows loads of 16, 8, 4 or 2 bytes
 };
 
-template <bool BF16>
 __device__ __forceinline__ uint4 f4_load_piece(const F4QuantParams& p, const uint16_t* row, int v) {
     const int k0 = v * 8;
-    if (p.vec_ok && k0 + 8 <= p.k) return __ldg(reinterpret_cast<const uint4*>(row + k0));
+    const uint16_t* at = row + k0;
+    if (k0 + 8 <= p.k) {                           // (which loads there are is the same for all rows)
+        if (p.vec_bytes == 16) return __ldg(reinterpret_cast<const uint4*>(at));
+        if (p.vec_bytes == 8) {
+            const uint2 a = __ldg(reinterpret_cast<const uint2*>(at)), b = __ldg(reinterpret_cast<const uint2*>(at) + 1);
+            return make_uint4(a.x, a.y, b.x, b.y);
+        }
+        if (p.vec_bytes == 4) {
+            const uint32_t* w = reinterpret_cast<const uint32_t*>(at);
+            return make_uint4(__ldg(w), __ldg(w + 1), __ldg(w + 2), __ldg(w + 3));
+        }
+    }
     uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-        if (k0 + j < p.k) w[j >> 1] |= static_cast<uint32_t>(__ldg(row + k0 + j)) << (16 * (j & 1));
+        if (k0 + j < p.k) w[j >> 1] |= static_cast<uint32_t>(__ldg(at + j)) << (16 * (j & 1));
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Largest |x| of a piece as 16-bit patterns (they order like integers), numbers only; `odd`: something else was there.
+// Largest |x| of a piece as a 16-bit pattern (they order like integers), numbers only; bit 16: something else was there.
 template <bool BF16>
-__device__ __forceinline__ uint32_t f4_piece_max(const uint4& d, bool& odd) {
+__device__ __forceinline__ uint32_t f4_piece_max(const uint4& d) {
     constexpr uint32_t kInf = BF16 ? 0x7F80u : 0x7C00u;
     uint32_t m = __vmaxu2(__vmaxu2(d.x & 0x7FFF7FFFu, d.y & 0x7FFF7FFFu), __vmaxu2(d.z & 0x7FFF7FFFu, d.w & 0x7FFF7FFFu));
     uint32_t one = max(m & 0xFFFFu, m >> 16);
-    odd = one >= kInf;
-    if (odd) {
+    if (one >= kInf) {
         const uint32_t w[4] = {d.x, d.y, d.z, d.w};
-        one = 0;
+        uint32_t most = 0;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const uint32_t b = (w[j >> 1] >> (16 * (j & 1))) & 0x7FFFu;
-            if (b < kInf) one = max(one, b);
+            if (b < kInf) most = max(most, b);
         }
+        one = most | 0x10000u;
     }
     return one;
 }
@@ -68,19 +80,25 @@ __device__ __forceinline__ float f4_bits_value(uint32_t bits) {
     return BF16 ? __uint_as_float(bits << 16) : __half2float(__ushort_as_half(static_cast<unsigned short>(bits)));
 }
 
+// What a row's pieces share.
+struct F4RowOut {
+    uint8_t* q;                  // the row's values, NULL beyond X
+    uint8_t* s;                  // byte 0 of the row's scales
+    int s_step;                  // bytes from one word of four scales to the next
+    float inv_row;               // FMT_E4M3: 1 / row factor ...
+    float pre;                   // ... times this: the row's numbers are multiplied by it first (bf16 rows far below 1)
+};
+
 // One piece: its block's scale (shared with the neighbouring threads of the block), codes and stores.
 template <int FMT, bool BF16>
-__device__ __forceinline__ void f4_emit(const F4QuantParams& p, const uint4& d, int row, int v, float inv_row) {
-    bool odd;
-    const uint32_t mine = f4_piece_max<BF16>(d, odd);
+__device__ __forceinline__ void f4_emit(const F4QuantParams& p, const F4RowOut& out, const uint4& d, uint32_t bits, int v) {
     constexpr int SHARE = f4_block(FMT) / 8;                            // threads of a block: 2 or 4
-    uint32_t bits = mine | (odd ? 0x10000u : 0u);
 #pragma unroll
     for (int o = 1; o < SHARE; o <<= 1) {
         const uint32_t other = __shfl_xor_sync(0xFFFFFFFFu, bits, o);
         bits = max(bits & 0xFFFFu, other & 0xFFFFu) | ((bits | other) & 0x10000u);
     }
-    odd = bits > 0xFFFFu;
+    const bool odd = bits > 0xFFFFu;
     const float amax = f4_bits_value<BF16>(bits & 0xFFFFu);
     uint32_t byte;
     float f[8];
@@ -96,36 +114,30 @@ __device__ __forceinline__ void f4_emit(const F4QuantParams& p, const uint4& d, 
         for (int j = 0; j < 8; ++j) f[j] = __fmul_rn(f[j], inv);
         if (odd) byte = 255;
     } else {
-        byte = __nv_cvt_float_to_fp8(__fdiv_rn(__fmul_rn(amax, inv_row), 6.0f), __NV_SATFINITE, __NV_E4M3);
-        const float s = e4m3_value(byte);
-        const float inv = s > 0.f ? __frcp_rn(s) : 0.f;
+        float a = amax;
+        if (BF16 && out.pre != 1.f) {                                   // the same for the whole row
+            a *= out.pre;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = __fsub_rn(__fadd_rn(__fmul_rn(__fmul_rn(f[j], inv_row), inv), 768.f), 768.f);
+            for (int j = 0; j < 8; ++j) f[j] *= out.pre;
+        }
+        // a / 6 rounded to the nearest: the quotient by multiplication, corrected by what it leaves
+        const float t = __fmul_rn(a, out.inv_row), guess = __fmul_rn(t, 1.f / 6.f);
+        byte = __nv_cvt_float_to_fp8(__fmaf_rn(__fmaf_rn(-6.f, guess, t), 1.f / 6.f, guess), __NV_SATFINITE, __NV_E4M3);
+        const float s = e4m3_value(byte);
+        const float inv = byte != 0 ? __fmul_rn(__fdividef(1.f, s), out.inv_row) : 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = __fsub_rn(__fmaf_rn(f[j], inv, 768.f), 768.f);
         if (odd) byte = 127;
     }
-    if (row < p.rows && v * 8 < p.k_padded) {
-        // the sign of a zero that was a negative number is kept, as the conversion does: it is the product's sign of zero
-        uint32_t codes = e2m1x8(f);
-        if constexpr (FMT == FMT_E4M3) {                                // 768 - 768 has lost it
-            const uint32_t w[4] = {d.x, d.y, d.z, d.w};
-            uint32_t neg = 0;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) neg |= ((w[j >> 1] >> (16 * (j & 1) + 15)) & 1u) << (4 * j + 3);
-            codes |= neg;
-        }
-        if (odd) codes = 0;
-        *reinterpret_cast<uint32_t*>(p.q + static_cast<size_t>(row) * (p.k_padded / 2) + v * 4) = codes;
-    }
+    uint32_t codes = e2m1x8(f);
+    if (odd) codes = 0;
+    if (out.q != nullptr && v * 8 < p.k_padded) *reinterpret_cast<uint32_t*>(out.q + v * 4) = codes;
     // four scales to a word: lanes of 4 consecutive blocks
     const int g = v / SHARE;
     uint32_t word = byte << (8 * (g & 3));
     word |= __shfl_xor_sync(0xFFFFFFFFu, word, SHARE);
     word |= __shfl_xor_sync(0xFFFFFFFFu, word, 2 * SHARE);
-    if (v < p.pieces && (v & (4 * SHARE - 1)) == 0) {
-        const size_t at = p.tiles_k ? (static_cast<size_t>(row >> 7) * p.tiles_k + (g >> 2)) * kF4TileBytes + (row & 31) * 16 + ((row >> 5) & 3) * 4
-                                    : static_cast<size_t>(row) * p.scale_pitch + g;
-        *reinterpret_cast<uint32_t*>(p.s + at) = word;
-    }
+    if (v < p.pieces && (v & (4 * SHARE - 1)) == 0) *reinterpret_cast<uint32_t*>(out.s + static_cast<size_t>(g >> 2) * out.s_step) = word;
 }
 
 // A group of blockDim.x threads (whole warps) per row, blockDim.y rows a CTA; a thread holds up to HELD pieces.
@@ -140,18 +152,25 @@ quantize_f4_kernel(const F4QuantParams p) {
     const uint16_t* src = p.x + static_cast<long long>(row) * p.ldx;
     const int mine = row < p.rows ? p.pieces : 0;  // rows beyond X: their scales are zeros
     uint4 held[HELD];
+    uint32_t most[HELD];
 #pragma unroll
     for (int i = 0; i < HELD; ++i) {
         const int v = tid + i * group;
-        held[i] = v < mine ? f4_load_piece<BF16>(p, src, v) : make_uint4(0, 0, 0, 0);
+        held[i] = v < mine ? f4_load_piece(p, src, v) : make_uint4(0, 0, 0, 0);
     }
-    float inv_row = 1.f;
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) most[i] = f4_piece_max<BF16>(held[i]);
+    F4RowOut out;
+    out.q = row < p.rows ? p.q + static_cast<size_t>(row) * (p.k_padded / 2) : nullptr;
+    out.s = p.tiles_k ? p.s + static_cast<size_t>(row >> 7) * p.tiles_k * kF4TileBytes + (row & 31) * 16 + ((row >> 5) & 3) * 4
+                      : p.s + static_cast<size_t>(row) * p.scale_pitch;
+    out.s_step = p.tiles_k ? kF4TileBytes : 4;
+    out.inv_row = out.pre = 1.f;
     if constexpr (FMT == FMT_E4M3) {
         uint32_t bits = 0;
-        bool odd;
 #pragma unroll
-        for (int i = 0; i < HELD; ++i) bits = max(bits, f4_piece_max<BF16>(held[i], odd));
-        for (int v = tid + HELD * group; v < mine; v += group) bits = max(bits, f4_piece_max<BF16>(f4_load_piece<BF16>(p, src, v), odd));
+        for (int i = 0; i < HELD; ++i) bits = max(bits, most[i] & 0xFFFFu);
+        for (int v = tid + HELD * group; v < mine; v += group) bits = max(bits, f4_piece_max<BF16>(f4_load_piece(p, src, v)) & 0xFFFFu);
         bits = __reduce_max_sync(0xFFFFFFFFu, bits);
         if (group > 32) {
             if ((tid & 31) == 0) warp_bits[tid >> 5] = bits;
@@ -160,18 +179,24 @@ quantize_f4_kernel(const F4QuantParams p) {
         }
         const float top = f4_bits_value<BF16>(bits);
         const int lg = static_cast<int>(__float_as_uint(top) >> 23);    // floor(log2 top) + 127
-        const int e = top == 0.f ? 127 : lg > 11 ? lg - 10 : 1;         // the row's factor is 2^(e - 127)
-        inv_row = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
+        int e = top == 0.f ? 127 : lg > 11 ? lg - 10 : 1;               // the row's factor is 2^(e - 127)
         if (tid == 0 && row < p.rows) p.row_scale[row] = __uint_as_float(static_cast<uint32_t>(e) << 23);
+        if (BF16 && e < 64) {                                           // 1 / factor times 1 / scale would leave fp32's range
+            out.pre = 0x1p64f;
+            e += 64;
+        }
+        out.inv_row = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
     }
     // whole warps go through every step together: neighbouring threads exchange their blocks' maxima
 #pragma unroll
     for (int i = 0; i < HELD; ++i) {
         const int v = tid + i * group;
-        if (v - (tid & 31) < p.pieces) f4_emit<FMT, BF16>(p, held[i], row, v, inv_row);
+        if (v - (tid & 31) < p.pieces) f4_emit<FMT, BF16>(p, out, held[i], most[i], v);
     }
-    for (int v = tid + HELD * group; v - (tid & 31) < p.pieces; v += group)
-        f4_emit<FMT, BF16>(p, v < mine ? f4_load_piece<BF16>(p, src, v) : make_uint4(0, 0, 0, 0), row, v, inv_row);   // second read hits L2
+    for (int v = tid + HELD * group; v - (tid & 31) < p.pieces; v += group) {
+        const uint4 d = v < mine ? f4_load_piece(p, src, v) : make_uint4(0, 0, 0, 0);                      // second read hits L2
+        f4_emit<FMT, BF16>(p, out, d, f4_piece_max<BF16>(d), v);
+    }
 }
 
 struct F4DequantParams {
@@ -182,54 +207,70 @@ struct F4DequantParams {
     long long ldo;
     int rows, k, k_padded;
     int tiles_k, scale_pitch;
-    int vec_ok;                  // the output allows 16-byte stores
+    int vec_bytes;               // the output allows stores of 16, 8, 4 or 2 bytes
 };
 
-// out = value * scale * row factor, rounded once.  A thread per 8 numbers: 4 bytes of codes, its block's scale, 16 or 32 bytes out.
+// out = value * scale * row factor, rounded once.  A thread per 8 columns and every fourth row of its CTA's: 4 bytes of codes, its block's scale,
+// 16 or 32 bytes out, four rows' loads in flight.  grid: (columns, rows)
+constexpr int kF4DequantRows = 4;
 template <int FMT, int TYPE>
 __global__ void __launch_bounds__(256)
 dequantize_f4_kernel(const F4DequantParams p) {
-    const int per_row = (p.k + 7) / 8;
-    const long long total = static_cast<long long>(p.rows) * per_row;
-    for (long long at = blockIdx.x * 256ll + threadIdx.x; at < total; at += gridDim.x * 256ll) {
-        const int row = static_cast<int>(at / per_row), v = static_cast<int>(at - static_cast<long long>(row) * per_row);
-        const uint32_t codes = __ldg(reinterpret_cast<const uint32_t*>(p.q + static_cast<size_t>(row) * (p.k_padded / 2) + v * 4));
-        const int g = v * 8 / f4_block(FMT);
-        const size_t sat = p.tiles_k ? (static_cast<size_t>(row >> 7) * p.tiles_k + (g >> 2)) * kF4TileBytes + (row & 31) * 16 + ((row >> 5) & 3) * 4 + (g & 3)
-                                     : static_cast<size_t>(row) * p.scale_pitch + g;
-        const float s = f4_scale_value<FMT>(__ldg(p.s + sat));
-        const float t = p.row_scale ? __ldg(p.row_scale + row) : 1.f;
-        uint32_t h[4];
-        e2m1x8_to_half(codes, h);
-        float f[8];
+    const int v = blockIdx.x * blockDim.x + threadIdx.x, k0 = v * 8;
+    if (k0 >= p.k) return;
+    const int g = k0 / f4_block(FMT);
+    for (int row0 = (blockIdx.y * blockDim.y + threadIdx.y) * kF4DequantRows; row0 < p.rows; row0 += gridDim.y * blockDim.y * kF4DequantRows) {
+        uint32_t codes[kF4DequantRows], byte[kF4DequantRows];
+        float t[kF4DequantRows];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float2 a = pair_to_float<false>(h[j]);
-            f[2 * j] = __fmul_rn(__fmul_rn(a.x, s), t);
-            f[2 * j + 1] = __fmul_rn(__fmul_rn(a.y, s), t);
+        for (int i = 0; i < kF4DequantRows; ++i) {
+            const int row = min(row0 + i, p.rows - 1);
+            codes[i] = __ldg(reinterpret_cast<const uint32_t*>(p.q + static_cast<size_t>(row) * (p.k_padded / 2) + v * 4));
+            byte[i] = __ldg(p.s + (p.tiles_k ? (static_cast<size_t>(row >> 7) * p.tiles_k + (g >> 2)) * kF4TileBytes + (row & 31) * 16 + ((row >> 5) & 3) * 4 + (g & 3)
+                                             : static_cast<size_t>(row) * p.scale_pitch + g));
+            t[i] = p.row_scale ? __ldg(p.row_scale + row) : 1.f;
         }
-        const int k0 = v * 8;
-        if constexpr (TYPE == TYPE_F32) {
-            float* dst = static_cast<float*>(p.out) + static_cast<long long>(row) * p.ldo + k0;
-            if (p.vec_ok && k0 + 8 <= p.k) {
-                reinterpret_cast<float4*>(dst)[0] = make_float4(f[0], f[1], f[2], f[3]);
-                reinterpret_cast<float4*>(dst)[1] = make_float4(f[4], f[5], f[6], f[7]);
-            } else {
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (k0 + j < p.k) dst[j] = f[j];
+        for (int i = 0; i < kF4DequantRows; ++i) {
+            const int row = row0 + i;
+            if (row >= p.rows) break;
+            const float s = f4_scale_value<FMT>(byte[i]);
+            uint32_t h[4];
+            e2m1x8_to_half(codes[i], h);
+            float f[8];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float2 a = pair_to_float<false>(h[j]);
+                f[2 * j] = __fmul_rn(__fmul_rn(a.x, s), t[i]);
+                f[2 * j + 1] = __fmul_rn(__fmul_rn(a.y, s), t[i]);
             }
-        } else {
-            constexpr bool BF16 = TYPE == TYPE_BF16;
-            uint16_t* dst = static_cast<uint16_t*>(p.out) + static_cast<long long>(row) * p.ldo + k0;
-            const uint32_t w[4] = {float_to_pair<BF16>(f[0], f[1]), float_to_pair<BF16>(f[2], f[3]), float_to_pair<BF16>(f[4], f[5]),
-                                   float_to_pair<BF16>(f[6], f[7])};
-            if (p.vec_ok && k0 + 8 <= p.k) {
-                *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+            constexpr int WORDS = TYPE == TYPE_F32 ? 8 : 4;
+            uint32_t w[WORDS];
+            if constexpr (TYPE == TYPE_F32) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) w[j] = __float_as_uint(f[j]);
             } else {
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (k0 + j < p.k) dst[j] = static_cast<uint16_t>(w[j >> 1] >> (16 * (j & 1)));
+                for (int j = 0; j < 4; ++j) w[j] = float_to_pair<TYPE == TYPE_BF16>(f[2 * j], f[2 * j + 1]);
+            }
+            constexpr int ELEM = TYPE == TYPE_F32 ? 4 : 2;
+            uint8_t* dst = static_cast<uint8_t*>(p.out) + (static_cast<long long>(row) * p.ldo + k0) * ELEM;
+            if (k0 + 8 <= p.k && p.vec_bytes == 16) {
+#pragma unroll
+                for (int j = 0; j < WORDS; j += 4) reinterpret_cast<uint4*>(dst)[j / 4] = make_uint4(w[j], w[j + 1], w[j + 2], w[j + 3]);
+            } else if (k0 + 8 <= p.k && p.vec_bytes == 8) {
+#pragma unroll
+                for (int j = 0; j < WORDS; j += 2) reinterpret_cast<uint2*>(dst)[j / 2] = make_uint2(w[j], w[j + 1]);
+            } else if (k0 + 8 <= p.k && p.vec_bytes == 4) {
+#pragma unroll
+                for (int j = 0; j < WORDS; ++j) reinterpret_cast<uint32_t*>(dst)[j] = w[j];
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    if (k0 + j >= p.k) break;
+                    if constexpr (TYPE == TYPE_F32) reinterpret_cast<uint32_t*>(dst)[j] = w[j];
+                    else reinterpret_cast<uint16_t*>(dst)[j] = static_cast<uint16_t>(w[j >> 1] >> (16 * (j & 1)));
+                }
             }
         }
     }
