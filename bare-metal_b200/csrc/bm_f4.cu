@@ -32,20 +32,15 @@ static bool aligned_to(const void* p, size_t n) { return reinterpret_cast<uintpt
 // ---- quantise ---------------------------------------------------------------------------
 template <int FMT, bool BF16>
 static int launch_quantize(const F4QuantParams& p, int sms, cudaStream_t stream) {
-    // Threads per row as in bm_quantize_rows_f16: four pieces a thread when there are many rows, one (two) when there are few.
-    auto group_for = [&](int held) { return ceil_div(ceil_div(p.pieces, held), 32) * 32; };
-    int held = 4, group = group_for(4);
-    if (p.rows <= sms) {
-        held = group_for(1) <= kF4QuantMaxThreads ? 1 : 2;
-        group = group_for(held);
-    }
-    const int most = held == 4 ? 512 : kF4QuantMaxThreads;
+    // Threads per row: two units a thread when there are many rows, one when there are few (the chip is empty and the length of a
+    // thread's own work is the latency), as far as 1024 threads reach.
+    const int held = p.rows <= sms ? 1 : 2, most = held == 2 ? 512 : kF4QuantMaxThreads;
+    int group = ceil_div(ceil_div(p.units, held), 32) * 32;
     if (group > most) group = most;                                // the rest of such a row is read twice
     const dim3 block(group, group == 32 ? 4 : 1);
     const dim3 grid(ceil_div(p.rows_padded, static_cast<int>(block.y)));
     if (held == 1) quantize_f4_kernel<FMT, BF16, 1><<<grid, block, 0, stream>>>(p);
-    else if (held == 2) quantize_f4_kernel<FMT, BF16, 2><<<grid, block, 0, stream>>>(p);
-    else quantize_f4_kernel<FMT, BF16, 4><<<grid, block, 0, stream>>>(p);
+    else quantize_f4_kernel<FMT, BF16, 2><<<grid, block, 0, stream>>>(p);
     BM_CUDA_TRY(cudaGetLastError());
     return BM_OK;
 }
@@ -266,14 +261,14 @@ int bm_quantize_f4(const void* X, int x_type, uint8_t* Q, uint8_t* S, float* row
     p.rows = R;
     p.k = K;
     p.k_padded = 2 * f4_row_bytes(K);
-    const int share = f4_block(format) / 8;
+    const int share = f4_block(format) / 16;
     if (scale_layout == BM_SCALE_TILED) {
         p.tiles_k = f4_tiles_k(K, format);
-        p.pieces = p.tiles_k * 4 * share;
+        p.units = p.tiles_k * 4 * share;
         p.rows_padded = ceil_div(R, 128) * 128;
     } else {
         p.scale_pitch = f4_scale_pitch(K, format);
-        p.pieces = p.scale_pitch * share;
+        p.units = p.scale_pitch * share;
         p.rows_padded = R;
     }
     p.vec_bytes = access_bytes(X, static_cast<size_t>(ldx) * 2);

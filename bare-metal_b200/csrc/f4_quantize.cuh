@@ -11,10 +11,10 @@
 // (a multiple of 1/4) or off every tie by more than 2^-13.  x * (1 / s) in fp32 is within 2^-20 of x / s; adding and
 // subtracting 768 rounds it to a multiple of 2^-14, which puts ties back on the tie and moves nothing across one.
 //
-// 2 bytes in and 1/2 + 1/16 (1/32) out per element.  A group of threads per row holds it in registers (16-byte pieces
-// of 8 numbers; two or four neighbouring threads share a block), so the row's maximum costs no second read.  What bounds it with
-// many rows is instructions as much as bytes, so an element gets one conversion, one FMA and one subtraction before the packing
-// conversion, and a piece's maximum is taken once.
+// 2 bytes in and 1/2 + 1/16 (1/32) out per element.  A group of threads per row holds it in registers, units of 16 numbers (a block,
+// or half of one), so the row's maximum costs no second read.  What bounds it with many rows is instructions as much as bytes: an
+// element gets one conversion, one FMA and one subtraction before the packing conversion, a unit its maximum once and its
+// scale once (8 numbers a thread and two threads a block took 171 instructions per 8).
 #pragma once
 #include "f4_format.cuh"
 
@@ -30,46 +30,50 @@ struct F4QuantParams {
     float* row_scale;            // FMT_E4M3
     int rows, rows_padded;       // rows of X; rows whose scales exist (whole tiles)
     int k, k_padded;             // row length; the same in whole 32s
-    int pieces;                  // pieces of 8 numbers that the stored scales of a row cover
+    int units;                   // units of 16 numbers that the stored scales of a row cover
     int tiles_k;                 // tiled scales: tiles along a row; 0: scales in rows
     int scale_pitch;             // scales in rows: bytes of a row
     int vec_bytes;               // X allows loads of 16, 8, 4 or 2 bytes
 };
 
-__device__ __forceinline__ uint4 f4_load_piece(const F4QuantParams& p, const uint16_t* row, int v) {
-    const int k0 = v * 8;
+struct F4Unit { uint32_t w[8]; };
+
+// unit v of a row, zeros beyond its end
+__device__ __forceinline__ F4Unit f4_load_unit(const F4QuantParams& p, const uint16_t* row, int v) {
+    F4Unit u;
+    const int k0 = v * 16;
     const uint16_t* at = row + k0;
-    if (k0 + 8 <= p.k) {                           // (which loads there are is the same for all rows)
-        if (p.vec_bytes == 16) return __ldg(reinterpret_cast<const uint4*>(at));
-        if (p.vec_bytes == 8) {
-            const uint2 a = __ldg(reinterpret_cast<const uint2*>(at)), b = __ldg(reinterpret_cast<const uint2*>(at) + 1);
-            return make_uint4(a.x, a.y, b.x, b.y);
-        }
-        if (p.vec_bytes == 4) {
-            const uint32_t* w = reinterpret_cast<const uint32_t*>(at);
-            return make_uint4(__ldg(w), __ldg(w + 1), __ldg(w + 2), __ldg(w + 3));
+    if (p.vec_bytes == 16 && k0 + 16 <= p.k) {
+        const uint4 a = __ldg(reinterpret_cast<const uint4*>(at)), b = __ldg(reinterpret_cast<const uint4*>(at) + 1);
+        u.w[0] = a.x; u.w[1] = a.y; u.w[2] = a.z; u.w[3] = a.w; u.w[4] = b.x; u.w[5] = b.y; u.w[6] = b.z; u.w[7] = b.w;
+    } else if (p.vec_bytes >= 4 && k0 + 16 <= p.k) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) u.w[j] = __ldg(reinterpret_cast<const uint32_t*>(at) + j);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            u.w[j] = k0 + 2 * j < p.k ? __ldg(at + 2 * j) : 0u;
+            if (k0 + 2 * j + 1 < p.k) u.w[j] |= static_cast<uint32_t>(__ldg(at + 2 * j + 1)) << 16;
         }
     }
-    uint32_t w[4] = {0, 0, 0, 0};
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-        if (k0 + j < p.k) w[j >> 1] |= static_cast<uint32_t>(__ldg(at + j)) << (16 * (j & 1));
-    return make_uint4(w[0], w[1], w[2], w[3]);
+    return u;
 }
 
-// Largest |x| of a piece as a 16-bit pattern (they order like integers), numbers only; bit 16: something else was there.
+// Largest |x| of a unit as a 16-bit pattern (they order like integers), numbers only; bit 16: something else was there.
 template <bool BF16>
-__device__ __forceinline__ uint32_t f4_piece_max(const uint4& d) {
+__device__ __forceinline__ uint32_t f4_unit_max(const F4Unit& u) {
     constexpr uint32_t kInf = BF16 ? 0x7F80u : 0x7C00u;
-    uint32_t m = __vmaxu2(__vmaxu2(d.x & 0x7FFF7FFFu, d.y & 0x7FFF7FFFu), __vmaxu2(d.z & 0x7FFF7FFFu, d.w & 0x7FFF7FFFu));
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = __vmaxu2(m, u.w[j] & 0x7FFF7FFFu);
     uint32_t one = max(m & 0xFFFFu, m >> 16);
     if (one >= kInf) {
-        const uint32_t w[4] = {d.x, d.y, d.z, d.w};
         uint32_t most = 0;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const uint32_t b = (w[j >> 1] >> (16 * (j & 1))) & 0x7FFFu;
-            if (b < kInf) most = max(most, b);
+            const uint32_t lo = u.w[j] & 0x7FFFu, hi = (u.w[j] >> 16) & 0x7FFFu;
+            if (lo < kInf) most = max(most, lo);
+            if (hi < kInf) most = max(most, hi);
         }
         one = most | 0x10000u;
     }
@@ -89,36 +93,37 @@ struct F4RowOut {
     float pre;                   // ... times this: the row's numbers are multiplied by it first (bf16 rows far below 1)
 };
 
-// One piece: its block's scale (shared with the neighbouring threads of the block), codes and stores.
+// One unit: its block's scale (FMT_E8M0: shared with the neighbouring thread), codes and stores.
 template <int FMT, bool BF16>
-__device__ __forceinline__ void f4_emit(const F4QuantParams& p, const F4RowOut& out, const uint4& d, uint32_t bits, int v) {
-    constexpr int SHARE = f4_block(FMT) / 8;                            // threads of a block: 2 or 4
-#pragma unroll
-    for (int o = 1; o < SHARE; o <<= 1) {
-        const uint32_t other = __shfl_xor_sync(0xFFFFFFFFu, bits, o);
+__device__ __forceinline__ void f4_emit(const F4QuantParams& p, const F4RowOut& out, const F4Unit& u, uint32_t bits, int v) {
+    constexpr int SHARE = f4_block(FMT) / 16;                           // threads of a block: 1 or 2
+    if constexpr (SHARE == 2) {
+        const uint32_t other = __shfl_xor_sync(0xFFFFFFFFu, bits, 1);
         bits = max(bits & 0xFFFFu, other & 0xFFFFu) | ((bits | other) & 0x10000u);
     }
     const bool odd = bits > 0xFFFFu;
     const float amax = f4_bits_value<BF16>(bits & 0xFFFFu);
     uint32_t byte;
-    float f[8];
-    {
-        const float2 a = pair_to_float<BF16>(d.x), b = pair_to_float<BF16>(d.y), c = pair_to_float<BF16>(d.z), e = pair_to_float<BF16>(d.w);
-        f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y; f[4] = c.x; f[5] = c.y; f[6] = e.x; f[7] = e.y;
+    float f[16];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float2 two = pair_to_float<BF16>(u.w[j]);
+        f[2 * j] = two.x;
+        f[2 * j + 1] = two.y;
     }
     if constexpr (FMT == FMT_E8M0) {
         const int lg = static_cast<int>(__float_as_uint(amax) >> 23);   // floor(log2 amax) + 127; 0 below 2^-126
         byte = lg > 2 ? lg - 2 : 0;
         const float inv = __uint_as_float((254u - byte) << 23);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = __fmul_rn(f[j], inv);
+        for (int j = 0; j < 16; ++j) f[j] = __fmul_rn(f[j], inv);
         if (odd) byte = 255;
     } else {
         float a = amax;
         if (BF16 && out.pre != 1.f) {                                   // the same for the whole row
             a *= out.pre;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) f[j] *= out.pre;
+            for (int j = 0; j < 16; ++j) f[j] *= out.pre;
         }
         // a / 6 rounded to the nearest: the quotient by multiplication, corrected by what it leaves
         const float t = __fmul_rn(a, out.inv_row), guess = __fmul_rn(t, 1.f / 6.f);
@@ -126,23 +131,23 @@ __device__ __forceinline__ void f4_emit(const F4QuantParams& p, const F4RowOut& 
         const float s = e4m3_value(byte);
         const float inv = byte != 0 ? __fmul_rn(__fdividef(1.f, s), out.inv_row) : 0.f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = __fsub_rn(__fmaf_rn(f[j], inv, 768.f), 768.f);
+        for (int j = 0; j < 16; ++j) f[j] = __fsub_rn(__fmaf_rn(f[j], inv, 768.f), 768.f);
         if (odd) byte = 127;
     }
-    uint32_t codes = e2m1x8(f);
-    if (odd) codes = 0;
-    if (out.q != nullptr && v * 8 < p.k_padded) *reinterpret_cast<uint32_t*>(out.q + v * 4) = codes;
+    const float lo[8] = {f[0], f[1], f[2], f[3], f[4], f[5], f[6], f[7]}, hi[8] = {f[8], f[9], f[10], f[11], f[12], f[13], f[14], f[15]};
+    const uint2 codes = odd ? make_uint2(0, 0) : make_uint2(e2m1x8(lo), e2m1x8(hi));
+    if (out.q != nullptr && v * 16 < p.k_padded) *reinterpret_cast<uint2*>(out.q + v * 8) = codes;
     // four scales to a word: lanes of 4 consecutive blocks
     const int g = v / SHARE;
     uint32_t word = byte << (8 * (g & 3));
     word |= __shfl_xor_sync(0xFFFFFFFFu, word, SHARE);
     word |= __shfl_xor_sync(0xFFFFFFFFu, word, 2 * SHARE);
-    if (v < p.pieces && (v & (4 * SHARE - 1)) == 0) *reinterpret_cast<uint32_t*>(out.s + static_cast<size_t>(g >> 2) * out.s_step) = word;
+    if (v < p.units && (v & (4 * SHARE - 1)) == 0) *reinterpret_cast<uint32_t*>(out.s + static_cast<size_t>(g >> 2) * out.s_step) = word;
 }
 
-// A group of blockDim.x threads (whole warps) per row, blockDim.y rows a CTA; a thread holds up to HELD pieces.
+// A group of blockDim.x threads (whole warps) per row, blockDim.y rows a CTA; a thread holds up to HELD units.
 template <int FMT, bool BF16, int HELD>
-__global__ void __launch_bounds__(HELD == 4 ? 512 : kF4QuantMaxThreads)
+__global__ void __launch_bounds__(HELD == 2 ? 512 : kF4QuantMaxThreads)
 quantize_f4_kernel(const F4QuantParams p) {
     __shared__ uint32_t warp_bits[kF4QuantMaxThreads / 32];
     const int row = blockIdx.x * blockDim.y + threadIdx.y;
@@ -150,16 +155,16 @@ quantize_f4_kernel(const F4QuantParams p) {
     pdl_launch_dependents();      // the GEMM behind this kernel may start its own set-up
     if (row >= p.rows_padded) return;              // whole warps: a CTA of several rows has one-warp groups
     const uint16_t* src = p.x + static_cast<long long>(row) * p.ldx;
-    const int mine = row < p.rows ? p.pieces : 0;  // rows beyond X: their scales are zeros
-    uint4 held[HELD];
+    const int mine = row < p.rows ? p.units : 0;   // rows beyond X: their scales are zeros
+    F4Unit held[HELD];
     uint32_t most[HELD];
 #pragma unroll
     for (int i = 0; i < HELD; ++i) {
         const int v = tid + i * group;
-        held[i] = v < mine ? f4_load_piece(p, src, v) : make_uint4(0, 0, 0, 0);
+        held[i] = v < mine ? f4_load_unit(p, src, v) : F4Unit{};
     }
 #pragma unroll
-    for (int i = 0; i < HELD; ++i) most[i] = f4_piece_max<BF16>(held[i]);
+    for (int i = 0; i < HELD; ++i) most[i] = f4_unit_max<BF16>(held[i]);
     F4RowOut out;
     out.q = row < p.rows ? p.q + static_cast<size_t>(row) * (p.k_padded / 2) : nullptr;
     out.s = p.tiles_k ? p.s + static_cast<size_t>(row >> 7) * p.tiles_k * kF4TileBytes + (row & 31) * 16 + ((row >> 5) & 3) * 4
@@ -170,7 +175,7 @@ quantize_f4_kernel(const F4QuantParams p) {
         uint32_t bits = 0;
 #pragma unroll
         for (int i = 0; i < HELD; ++i) bits = max(bits, most[i] & 0xFFFFu);
-        for (int v = tid + HELD * group; v < mine; v += group) bits = max(bits, f4_piece_max<BF16>(f4_load_piece(p, src, v)) & 0xFFFFu);
+        for (int v = tid + HELD * group; v < mine; v += group) bits = max(bits, f4_unit_max<BF16>(f4_load_unit(p, src, v)) & 0xFFFFu);
         bits = __reduce_max_sync(0xFFFFFFFFu, bits);
         if (group > 32) {
             if ((tid & 31) == 0) warp_bits[tid >> 5] = bits;
@@ -191,11 +196,11 @@ quantize_f4_kernel(const F4QuantParams p) {
 #pragma unroll
     for (int i = 0; i < HELD; ++i) {
         const int v = tid + i * group;
-        if (v - (tid & 31) < p.pieces) f4_emit<FMT, BF16>(p, out, held[i], most[i], v);
+        if (v - (tid & 31) < p.units) f4_emit<FMT, BF16>(p, out, held[i], most[i], v);
     }
-    for (int v = tid + HELD * group; v - (tid & 31) < p.pieces; v += group) {
-        const uint4 d = v < mine ? f4_load_piece(p, src, v) : make_uint4(0, 0, 0, 0);                      // second read hits L2
-        f4_emit<FMT, BF16>(p, out, d, f4_piece_max<BF16>(d), v);
+    for (int v = tid + HELD * group; v - (tid & 31) < p.units; v += group) {
+        const F4Unit u = v < mine ? f4_load_unit(p, src, v) : F4Unit{};                                    // second read hits L2
+        f4_emit<FMT, BF16>(p, out, u, f4_unit_max<BF16>(u), v);
     }
 }
 
