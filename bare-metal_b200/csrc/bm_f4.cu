@@ -32,15 +32,15 @@ static bool aligned_to(const void* p, size_t n) { return reinterpret_cast<uintpt
 // ---- quantise ---------------------------------------------------------------------------
 template <int FMT, bool BF16>
 static int launch_quantize(const F4QuantParams& p, int sms, cudaStream_t stream) {
-    // Threads per row: two units a thread when there are many rows, one when there are few (the chip is empty and the length of a
+    // Threads per row: four units a thread when there are many rows, one when there are few (the chip is empty and the length of a
     // thread's own work is the latency), as far as 1024 threads reach.
-    const int held = p.rows <= sms ? 1 : 2, most = held == 2 ? 512 : kF4QuantMaxThreads;
+    const int held = p.rows <= sms ? 1 : 4, most = held == 4 ? 512 : kF4QuantMaxThreads;
     int group = ceil_div(ceil_div(p.units, held), 32) * 32;
     if (group > most) group = most;                                // the rest of such a row is read twice
     const dim3 block(group, group == 32 ? 4 : 1);
     const dim3 grid(ceil_div(p.rows_padded, static_cast<int>(block.y)));
     if (held == 1) quantize_f4_kernel<FMT, BF16, 1><<<grid, block, 0, stream>>>(p);
-    else quantize_f4_kernel<FMT, BF16, 2><<<grid, block, 0, stream>>>(p);
+    else quantize_f4_kernel<FMT, BF16, 4><<<grid, block, 0, stream>>>(p);
     BM_CUDA_TRY(cudaGetLastError());
     return BM_OK;
 }

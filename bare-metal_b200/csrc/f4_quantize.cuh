@@ -147,7 +147,7 @@ __device__ __forceinline__ void f4_emit(const F4QuantParams& p, const F4RowOut& 
 
 // A group of blockDim.x threads (whole warps) per row, blockDim.y rows a CTA; a thread holds up to HELD units.
 template <int FMT, bool BF16, int HELD>
-__global__ void __launch_bounds__(HELD == 2 ? 512 : kF4QuantMaxThreads)
+__global__ void __launch_bounds__(HELD == 4 ? 512 : kF4QuantMaxThreads)
 quantize_f4_kernel(const F4QuantParams p) {
     __shared__ uint32_t warp_bits[kF4QuantMaxThreads / 32];
     const int row = blockIdx.x * blockDim.y + threadIdx.y;
