@@ -87,11 +87,12 @@ static int launch_f4_inst(const F4Operands& o, F4GemmParams& p, DeviceState* dev
     using Cfg = F4Cfg<PAIR, FMT>;
     const size_t elem = TYPE == TYPE_F32 ? 4 : 2;
     const int pitch = f4_row_bytes(o.K);
-    CUtensorMap ma, msa, mb, msb, mo;
+    CUtensorMap ma, msa, mb, msb, mb_half, msb_half, mo;
     if (int rc = make_tensor_map_u8(&ma, o.a, pitch, o.M, pitch, 128, 128, true)) return rc;
     if (int rc = make_tensor_map_u8(&mb, o.b, pitch, o.N, pitch, 128, 128, true)) return rc;
     if (int rc = scale_map(&msa, o.sa, o.M, o.K, FMT, 1)) return rc;
     if (int rc = scale_map(&msb, o.sb, o.N, o.K, FMT, Cfg::BN / 128)) return rc;
+    p.pair_ok = access_bytes(p.out, static_cast<size_t>(p.ld) * elem) >= 4;
     mo = ma;                                         // placeholder unless the output qualifies for TMA stores
     if (aligned16(p.out) && (static_cast<size_t>(p.ld) * elem) % 16 == 0 && opt(OPT_TMA_STORE) != 0) {
         if (int rc = make_tensor_map_out(&mo, p.out, o.N, o.M, static_cast<size_t>(p.ld) * elem, static_cast<int>(elem))) return rc;
@@ -105,12 +106,21 @@ static int launch_f4_inst(const F4Operands& o, F4GemmParams& p, DeviceState* dev
     if (tiles > 0x7FFFFFFF) return fail_msg(BM_ERR_TOO_LARGE, "more than 2^31 output tiles");
     const int slots = PAIR ? dev->sm_count / 2 : dev->sm_count;
     const int units = tiles < slots ? static_cast<int>(tiles) : slots;
+    p.tail_first = static_cast<int>(tiles);
+    mb_half = mb;
+    msb_half = msb;
+    const int rest = static_cast<int>(tiles % units);
+    if (PAIR && tiles > units && rest > 0 && 2 * rest <= units && opt(OPT_TAIL_NARROW) != 0) {
+        p.tail_first -= rest;
+        if (int rc = make_tensor_map_u8(&mb_half, o.b, pitch, o.N, pitch, 128, 64, true)) return rc;
+        if (int rc = scale_map(&msb_half, o.sb, o.N, o.K, FMT, 1)) return rc;
+    }
     if (PAIR) p.group_m = p.tiles_m >= 2 * p.tiles_n && p.tiles_m >= 16 ? 8 : 0;      // as for the int8 pair kernel
     auto kern = f4_gemm_kernel<PAIR, FMT, TYPE>;
     static ConfiguredFlags flags;
     if (int rc = ensure_smem_limit(flags, kern, Cfg::SMEM_BYTES)) return rc;
     BM_CUDA_TRY(launch_pdl(kern, dim3(PAIR ? 2 * units : units), dim3(kDenseThreads), Cfg::SMEM_BYTES, stream, PAIR ? 2 : 1, ma, msa, mb,
-                           msb, mo, p));
+                           msb, mb_half, msb_half, mo, p));
     return BM_OK;
 }
 template <bool PAIR>

@@ -13,6 +13,8 @@
 // igemm_sparse_pair.cuh.  Copies into tensor memory and MMAs of one thread execute in the order of their issue, so the
 // scales of the next stage may follow the MMAs that read the ones before.
 //
+// Where at most half of the pairs would work in the last wave, its tiles are cut into two halves of 128 columns for two pairs.
+//
 // What bounds it: an SM needs 128 x 256 x 64 MACs = 128 clocks an MMA (512 a stage) and 38 KiB of operands a stage, 76 B/clk.
 #pragma once
 #include "epilogue.cuh"
@@ -102,7 +104,9 @@ struct F4GemmParams {
     const float* col_scale;      // rb, or NULL for ones
     int tiles_m, tiles_n, k_blocks;
     int group_m;                 // tile order, as DenseParams::group_m
+    int tail_first;              // tiles from here on are computed as two halves of 128 columns by different pairs
     int tma_ok;                  // the output is stored through TMA
+    int pair_ok;                 // the output allows 4-byte stores at even columns
     int* status;
 };
 
@@ -133,6 +137,27 @@ __device__ __forceinline__ uint4 f4_convert16(const uint32_t* r, const float* co
     }
 }
 
+// A staged box (32 rows of 128 bytes, 128-byte swizzle) to the output, a row at a time: 128 bytes side by side by the 32 lanes.  (Each lane
+// storing its own row, element by element, took 33 us for 777 x 2260 x 1000 in fp16.)
+template <class T>
+__device__ __forceinline__ void f4_copy_box(const F4GemmParams& p, uint32_t stage_smem, int row0, int col0, int lane) {
+    constexpr int PER = 4 / sizeof(T);
+    const int col = col0 + lane * PER, rows = min(32, p.rows - row0);
+    T* dst = reinterpret_cast<T*>(p.out) + static_cast<long long>(row0) * p.ld + col;
+#pragma unroll 4
+    for (int r = 0; r < rows; ++r, dst += p.ld) {
+        uint32_t w;
+        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(stage_smem + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4) : "memory");
+        if (PER == 1 || p.pair_ok) {
+            if (col + PER <= p.cols) { *reinterpret_cast<uint32_t*>(dst) = w; continue; }
+        }
+        const T* t = reinterpret_cast<const T*>(&w);
+#pragma unroll
+        for (int j = 0; j < PER; ++j)
+            if (col + j < p.cols) dst[j] = t[j];
+    }
+}
+
 // Drains NC columns of 32 rows (one per lane) in chunks of 32.  `reverse`: the upper half of the chunks first (NC = 128).
 // `first_half` is called once, when the first 64 columns have left the accumulator.
 template <int TYPE, int NC, class Hook>
@@ -147,32 +172,20 @@ __device__ __forceinline__ void f4_drain(const F4GemmParams& p, const CUtensorMa
     auto chunk_at = [&](int i) { return reverse ? i ^ (CHUNKS / 2) : i; };
     auto live_at = [&](int i) { return col0 + chunk_at(i) * 32 < p.cols; };             // warp-uniform
     uint32_t rr[2][32];
-    if (live_at(0)) tmem_ld_32x32(taddr + chunk_at(0) * 32, rr[0]);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        if (live_at(i)) tmem_ld_32x32(taddr + chunk_at(i) * 32, rr[i]);
+    tmem_ld_wait();
+    first_half();                                               // before anything is converted: the next tile's MMAs may wait for it
 #pragma unroll
     for (int i = 0; i < CHUNKS; ++i) {
         const int c = chunk_at(i);
         const bool live = live_at(i);
-        if (live) tmem_ld_wait();
-        if (i == 1) first_half();
-        if (i + 1 < CHUNKS && live_at(i + 1)) tmem_ld_32x32(taddr + chunk_at(i + 1) * 32, rr[(i + 1) & 1]);
+        if (i >= 2 && live) tmem_ld_wait();
         const uint32_t* r = rr[i & 1];
         const int box_c0 = col0 + (c / CHUNKS_PER_BOX) * CHUNKS_PER_BOX * 32;
-        // TMA writes whole pieces of 16 bytes: a box that ends inside one is stored element by element
-        if (!(p.tma_ok && (p.cols % PER == 0 || box_c0 + CHUNKS_PER_BOX * 32 <= p.cols))) {
-            const int row = row0 + lane;
-            if (live && row < p.rows) {
-                T* dst = reinterpret_cast<T*>(p.out) + static_cast<long long>(row) * p.ld + col0 + c * 32;
-#pragma unroll
-                for (int v = 0; v < PIECES; ++v) {
-                    const uint4 o = f4_convert16<TYPE>(r + v * PER, strip + c * 32 + v * PER, row_s);
-                    const T* t = reinterpret_cast<const T*>(&o);
-#pragma unroll
-                    for (int j = 0; j < PER; ++j)
-                        if (col0 + c * 32 + v * PER + j < p.cols) dst[v * PER + j] = t[j];
-                }
-            }
-            continue;
-        }
+        // TMA writes whole pieces of 16 bytes: a box that ends inside one, or an output that TMA cannot store, is copied by the warp
+        const bool by_tma = p.tma_ok && (p.cols % PER == 0 || box_c0 + CHUNKS_PER_BOX * 32 <= p.cols);
         if (live) {
             if (i % CHUNKS_PER_BOX == 0) {
                 if (lane == 0) bulk_wait_read_all();            // the box before this one has been fetched
@@ -187,23 +200,56 @@ __device__ __forceinline__ void f4_drain(const F4GemmParams& p, const CUtensorMa
                              : "memory");
             }
         }
+        if (i + 2 < CHUNKS && live_at(i + 2)) tmem_ld_32x32(taddr + chunk_at(i + 2) * 32, rr[i & 1]);
         if (i % CHUNKS_PER_BOX == CHUNKS_PER_BOX - 1 && box_c0 < p.cols && row0 < p.rows) {
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) {
-                tma_store_2d(map, stage_smem, box_c0, row0);
-                bulk_commit_group();
+            if (by_tma) {
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                    tma_store_2d(map, stage_smem, box_c0, row0);
+                    bulk_commit_group();
+                }
+            } else {
+                __syncwarp();
+                f4_copy_box<T>(p, stage_smem, row0, box_c0, lane);
+                __syncwarp();
             }
         }
     }
 }
 
+// Work of one unit (a pair or a CTA): tiles unit, unit + units, ... below `tail_first`, then, on pairs, half the columns of one tile of
+// the partly filled last wave.
+struct F4Work {
+    int tile, half;              // half < 0: the whole tile
+};
+struct F4WorkIter {
+    int next_tile, units, tiles, tail_first, unit;
+    bool tail_done;
+    __device__ F4WorkIter(int unit_, int units_, const F4GemmParams& p)
+        : next_tile(unit_), units(units_), tiles(p.tiles_m * p.tiles_n), tail_first(p.tail_first), unit(unit_), tail_done(false) {}
+    __device__ bool next(F4Work& w) {
+        w.half = -1;
+        if (next_tile < tail_first) {
+            w.tile = next_tile;
+            next_tile += units;
+            return true;
+        }
+        if (tail_done || unit >= (tiles - tail_first) * 2) return false;
+        tail_done = true;
+        w.tile = tail_first + unit / 2;
+        w.half = unit % 2;
+        return true;
+    }
+};
+
 // map_a, map_b: packed values as byte maps, boxes of 128 bytes x 128 rows.  map_sa, map_sb: tiled scales as [128-row tile]
-// [4 * tiles_k rows][128 bytes]; what a box reaches beyond K or beyond the last row tile arrives as zeros.
+// [4 * tiles_k rows][128 bytes]; map_b_half, map_sb_half: the same for half a tile (PAIR).  What a box reaches beyond K or beyond the last row tile arrives as zeros.
 template <bool PAIR, int FMT, int TYPE>
 __global__ void __launch_bounds__(kDenseThreads, 1)
 f4_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_sa,
                const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_sb,
+               const __grid_constant__ CUtensorMap map_b_half, const __grid_constant__ CUtensorMap map_sb_half,
                const __grid_constant__ CUtensorMap map_out, const F4GemmParams p) {
     using Cfg = F4Cfg<PAIR, FMT>;
     constexpr int STAGES = Cfg::STAGES, KT = Cfg::KT;
@@ -228,7 +274,6 @@ f4_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     const uint32_t rank = PAIR ? cluster_ctarank() : 0u;                // 0 = leader
     const int unit = PAIR ? blockIdx.x >> 1 : blockIdx.x;
     const int units = PAIR ? gridDim.x >> 1 : gridDim.x;
-    const int num_tiles = p.tiles_m * p.tiles_n;
     auto tile_coords = [&](int tile, int& tm, int& tn) {
         if (p.group_m <= 0) { tm = tile % p.tiles_m; tn = tile / p.tiles_m; return; }
         const int band_tiles = p.group_m * p.tiles_n;
@@ -276,9 +321,11 @@ f4_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         prefetch_tensormap(&map_sb);
         uint32_t stage = 0, phase = 0;
         bool ok = true;
-        for (int tile = unit; ok && tile < num_tiles; tile += units) {
+        F4WorkIter work(unit, units, p);
+        F4Work w;
+        while (ok && work.next(w)) {
             int tm, tn;
-            tile_coords(tile, tm, tn);
+            tile_coords(w.tile, tm, tn);
             const int am = tm * (Cfg::ROWS / 128) + static_cast<int>(rank);        // 128-row blocks of A and W
             const int bn = tn * (Cfg::BN / 128) + static_cast<int>(rank);
             for (int kb = 0; kb < p.k_blocks; ++kb) {
@@ -288,11 +335,14 @@ f4_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                     const uint32_t sfa_dst = sfa_smem0 + stage * Cfg::SFA_BYTES, sfb_dst = sfb_smem0 + stage * Cfg::SFB_BYTES;
                     if constexpr (PAIR) {
                         const uint32_t bar = mapa_shared(full_bar(stage), 0);
-                        if (rank == 0) mbar_expect_tx(full_bar(stage), 2 * Cfg::STAGE_BYTES);
+                        const bool whole = w.half < 0;
+                        if (rank == 0)
+                            mbar_expect_tx(full_bar(stage), 2 * (whole ? Cfg::STAGE_BYTES : Cfg::STAGE_BYTES - (Cfg::AB_BYTES + Cfg::SFB_BYTES) / 2));
                         tma_load_2d_pair(a_dst, &map_a, bar, kb * 128, am * 128);
-                        tma_load_2d_pair(b_dst, &map_b, bar, kb * 128, bn * 128);
+                        tma_load_2d_pair(b_dst, whole ? &map_b : &map_b_half, bar, kb * 128,
+                                         whole ? bn * 128 : tn * 256 + w.half * 128 + static_cast<int>(rank) * 64);
                         tma_load_3d_pair(sfa_dst, &map_sa, bar, 0, kb * KT * 4, am);
-                        tma_load_3d_pair(sfb_dst, &map_sb, bar, 0, kb * KT * 4, tn * 2);
+                        tma_load_3d_pair(sfb_dst, whole ? &map_sb : &map_sb_half, bar, 0, kb * KT * 4, whole ? tn * 2 : tn * 2 + w.half);
                     } else {
                         const uint32_t bar = full_bar(stage);
                         mbar_expect_tx(bar, Cfg::STAGE_BYTES);
@@ -311,13 +361,16 @@ f4_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         if (rank == 0) {
             uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0, sf_buf = 0;
             [[maybe_unused]] uint32_t overlap_phase = 0;
-            bool ok = true;
-            for (int tile = unit; ok && tile < num_tiles; tile += units) {
+            bool ok = true, first = true;
+            F4WorkIter work(unit, units, p);
+            F4Work w;
+            while (ok && work.next(w)) {
                 if (!warp_bounded_wait(acc_empty_bar(acc), acc_phase ^ 1u, abort_flag, p.status, DEV_TIMEOUT_MMA_ACC_EMPTY)) { ok = false; break; }
-                if (PAIR && tile != unit) {
+                if (PAIR && !first) {
                     if (!warp_bounded_wait(overlap_bar, overlap_phase, abort_flag, p.status, DEV_TIMEOUT_MMA_ACC_EMPTY)) { ok = false; break; }
                     overlap_phase ^= 1u;
                 }
+                first = false;
                 tc_fence_after_sync();
                 const uint32_t d_tmem = tmem_base + acc * Cfg::ACC_STRIDE;
                 for (int kb = 0; kb < p.k_blocks; ++kb) {
@@ -332,15 +385,16 @@ f4_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                             tmem_cp_scales<PAIR>(sfa_tmem + t * 4, sfa_desc + t * (kF4TileBytes >> 4));
 #pragma unroll
                             for (int r = 0; r < Cfg::BN / 128; ++r)
-                                tmem_cp_scales<PAIR>(sfb_tmem + t * (Cfg::BN / 32) + r * 4, sfb_desc + (r * KT + t) * (kF4TileBytes >> 4));
+                                if (r == 0 || w.half < 0) tmem_cp_scales<PAIR>(sfb_tmem + t * (Cfg::BN / 32) + r * 4, sfb_desc + (r * KT + t) * (kF4TileBytes >> 4));
                         }
                         const uint64_t a_desc = make_smem_desc(a_smem0 + stage * Cfg::AB_BYTES, 0, 1024, SWIZZLE_128B_DESC);
                         const uint64_t b_desc = make_smem_desc(b_smem0 + stage * Cfg::AB_BYTES, 0, 1024, SWIZZLE_128B_DESC);
 #pragma unroll
                         for (int ks = 0; ks < 4; ++ks) {
                             const int t = ks * KT / 4;                                 // scale tile of these 64 of K
-                            constexpr uint32_t idesc0 = make_idesc_f4<FMT>(Cfg::ROWS, Cfg::BN, 0), idesc2 = make_idesc_f4<FMT>(Cfg::ROWS, Cfg::BN, 2);
-                            mma_f4<PAIR, FMT>(d_tmem, a_desc + ks * 2, b_desc + ks * 2, FMT == FMT_E8M0 && (ks & 1) ? idesc2 : idesc0,
+                            const int byte = FMT == FMT_E8M0 ? (ks & 1) * 2 : 0;
+                            const uint32_t idesc = PAIR && w.half >= 0 ? make_idesc_f4<FMT>(Cfg::ROWS, Cfg::BN / 2, byte) : make_idesc_f4<FMT>(Cfg::ROWS, Cfg::BN, byte);
+                            mma_f4<PAIR, FMT>(d_tmem, a_desc + ks * 2, b_desc + ks * 2, idesc,
                                               sfa_tmem + t * 4, sfb_tmem + t * (Cfg::BN / 32), (kb | ks) != 0 ? 1u : 0u);
                         }
                         if constexpr (PAIR) {
@@ -383,14 +437,17 @@ f4_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         float* strip = reinterpret_cast<float*>(smem_gen + Cfg::STRIP_OFFSET) + (warp - 2) * Cfg::NC;
         const uint32_t my_stage = smem_base + Cfg::STORE_OFFSET + (warp - 2) * kStoreBoxBytes;
         uint32_t acc = 0, acc_phase = 0;
-        for (int tile = unit; tile < num_tiles; tile += units) {
+        F4WorkIter work(unit, units, p);
+        F4Work w;
+        while (work.next(w)) {
             int tm, tn;
-            tile_coords(tile, tm, tn);
+            tile_coords(w.tile, tm, tn);
             const int row0 = tm * Cfg::ROWS + static_cast<int>(rank) * 128 + quarter * 32;
-            const int col0 = tn * Cfg::BN + half * Cfg::NC;
+            const int columns = w.half < 0 ? Cfg::NC : Cfg::NC / 2;          // of this warp
+            const int col0 = tn * Cfg::BN + (w.half < 0 ? 0 : w.half * Cfg::NC) + half * columns;
             __syncwarp();                                        // the strip has been read
 #pragma unroll
-            for (int i = lane; i < Cfg::NC; i += 32) {
+            for (int i = lane; i < Cfg::NC; i += 32) {                       // (half a tile does not use all)
                 const int c = col0 + i;
                 strip[i] = c < p.cols && p.col_scale ? __ldg(p.col_scale + c) : 1.f;
             }
@@ -399,7 +456,7 @@ f4_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
             const float row_s = row < p.rows && p.row_scale ? __ldg(p.row_scale + row) : 1.f;
             if (!bounded_wait(acc_full_bar(acc), acc_phase, abort_flag, p.status, DEV_TIMEOUT_EPI_ACC_FULL)) break;
             tc_fence_after_sync();
-            const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + acc * Cfg::ACC_STRIDE + half * Cfg::NC;
+            const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + acc * Cfg::ACC_STRIDE + half * columns;
             // the columns both accumulators of a pair share: the last 64 of the first, the first 64 of the second one
             const bool has_overlap = PAIR && half != static_cast<int>(acc);
             auto overlap_read = [&] {
@@ -408,7 +465,8 @@ f4_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                 __syncwarp();
                 if (lane == 0) mbar_arrive_cluster(mapa_shared(overlap_bar, 0));
             };
-            f4_drain<TYPE, Cfg::NC>(p, &map_out, taddr, row0, lane, col0, strip, row_s, my_stage, PAIR && half == 1, overlap_read);
+            if (PAIR && w.half >= 0) f4_drain<TYPE, 64>(p, &map_out, taddr, row0, lane, col0, strip, row_s, my_stage, false, NoHook{});      // the last unit
+            else f4_drain<TYPE, Cfg::NC>(p, &map_out, taddr, row0, lane, col0, strip, row_s, my_stage, PAIR && half == 1, overlap_read);
             tc_fence_before_sync();
             __syncwarp();
             if (lane == 0) {

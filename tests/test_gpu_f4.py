@@ -169,6 +169,22 @@ def test_product_is_the_same_on_every_call(kernel, M, fmt):
     assert all(torch.equal(outs[0], o) for o in outs[1:])
 
 
+@pytest.mark.parametrize("fmt", [ig.BM_F4_E8M0, ig.BM_F4_E4M3])
+@pytest.mark.parametrize("M,N", [(2560, 2048), (2500, 2300), (2304, 2432)])                 # 80 and 90 pair tiles: the last wave of 74 pairs is cut up
+def test_product_with_a_partly_filled_last_wave(M, N, fmt):
+    K = 800
+    X, W, a, b = product_inputs(M, N, K, fmt, seed=6)
+    for dtype in (torch.float16, torch.float32):
+        D = torch.full((M, N), 7.0, dtype=dtype, device=dev())
+        with options(f4_kernel=3):
+            ig.f4_linear(*X, *W, D, M, N, K, fmt)
+            with options(tail_narrow=0):
+                whole = ig.f4_linear(*X, *W, torch.empty_like(D), M, N, K, fmt)
+        assert torch.equal(D, whole)
+        check_product(D, a, b)
+    assert_clean_status()
+
+
 @pytest.mark.parametrize("kernel,M", [(1, 9), (2, 150), (3, 260)])
 @pytest.mark.parametrize("fmt", [ig.BM_F4_E8M0, ig.BM_F4_E4M3])
 def test_nan_scales_reach_their_rows_and_columns_only(kernel, M, fmt):
