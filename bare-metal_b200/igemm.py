@@ -17,6 +17,8 @@ plus the entry points the B200 workloads add: igemm_i32, w8a8_linear, sparse wei
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import _lib
@@ -307,62 +309,87 @@ def _here(t: torch.Tensor, name: str) -> torch.Tensor:
     """A CUDA tensor of the current device (kernels run on its current stream)."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise BmError(f"{name} must be a CUDA tensor")
-    if t.get_device() != torch.cuda.current_device():
+    if t.get_device() != _device():
         raise BmError(f"{name} must be on the current device")
     return t
 
 
-def _buffer(t: torch.Tensor, dtype, numel: int, name: str) -> int:
+def _device() -> int:
+    try:
+        return torch._C._cuda_getDevice()                # 0.1 us against 0.5
+    except AttributeError:
+        return torch.cuda.current_device()
+
+
+def _buffer(t: torch.Tensor, dtype, numel: int, name: str, device: int) -> int:
+    """Address of a contiguous tensor with at least `numel` elements on `device`, the current one."""
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == device and t.is_contiguous() and t.numel() >= numel:
+        return t.data_ptr()
     if _here(t, name).dtype != dtype:
         raise BmError(f"{name} must have dtype {dtype}, got {t.dtype}")
-    if not t.is_contiguous() or t.numel() < numel:
-        raise BmError(f"{name} must be contiguous and hold {numel} elements")
-    return t.data_ptr()
+    raise BmError(f"{name} must be contiguous and hold {numel} elements")
 
 
 def _f4_rows(t: torch.Tensor, name: str) -> int:
     """Elements between the rows of a matrix whose rows are contiguous."""
-    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
-        raise BmError(f"{name} must be a matrix with unit stride along its rows")
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    if t.dim() != 2:
+        raise BmError(f"{name} must be a matrix")
+    (rows, columns), (pitch, step) = t.shape, t.stride()
+    if columns > 1 and step != 1:
+        raise BmError(f"{name} must have unit stride along its rows")
+    return pitch if rows > 1 else columns
 
 
-def _f4_matrix(q, s, r, R, K, fmt, layout, name):
-    """Pointers of the three parts of a 4-bit matrix."""
-    if fmt not in _F4_BLOCK:
-        raise BmError(f"unknown 4-bit format tag {fmt}")
+@functools.lru_cache(maxsize=4096)
+def _f4_bytes(R, K, fmt, layout):
+    """Bytes of the values and of the scales of an R x K matrix."""
     L = _lib.load()
-    return (_buffer(q, torch.uint8, L.bm_f4_value_bytes(R, K), f"{name} values"),
-            _buffer(s, torch.uint8, L.bm_f4_scale_bytes(R, K, fmt, layout), f"{name} scales"),
-            None if r is None else _buffer(r, torch.float32, R, f"{name} row factors"))
+    values, scales = L.bm_f4_value_bytes(R, K), L.bm_f4_scale_bytes(R, K, fmt, layout)
+    if not values or not scales:
+        raise BmError(f"no 4-bit matrix has {R} x {K} elements, format tag {fmt} and scale layout tag {layout}")
+    return values, scales
+
+
+def _f4_matrix(q, s, r, R, K, fmt, layout, name, device):
+    """Pointers of the three parts of a 4-bit matrix."""
+    values, scales = _f4_bytes(R, K, fmt, layout)
+    return (_buffer(q, torch.uint8, values, name, device), _buffer(s, torch.uint8, scales, name, device),
+            None if r is None else _buffer(r, torch.float32, R, name, device))
+
+
+def _new(like: torch.Tensor, shape, dtype) -> torch.Tensor:
+    """An uninitialised plain tensor on the device of `like`."""
+    if type(like) is torch.Tensor:                       # 1.6 us an allocation against 2.3, but a subclass would get its own type
+        return like.new_empty(shape, dtype=dtype)
+    return torch.empty(shape, dtype=dtype, device=like.device)
 
 
 def quantize_f4(X, fmt=BM_F4_E4M3, scale_layout=BM_SCALE_TILED):
     """Rows of a fp16 / bf16 matrix to 4 bits: (values uint8 [R, ceil(K/32)*16], scales uint8 — [R, pitch] in rows, 1-D tiled —,
     row factors fp32 [R], None for BM_F4_E8M0)."""
-    L = _lib.load()
     if _here(X, "X").dtype not in (torch.float16, torch.bfloat16):
         raise BmError("X must be float16 or bfloat16")
     ldx = _f4_rows(X, "X")
     R, K = X.shape
-    nbytes = L.bm_f4_scale_bytes(R, K, fmt, scale_layout)
-    q = torch.empty((R, (K + 31) // 32 * 16), dtype=torch.uint8, device=X.device)
-    s = torch.empty((R, nbytes // R) if scale_layout == BM_SCALE_ROWS and R else nbytes, dtype=torch.uint8, device=X.device)
-    r = torch.empty(R, dtype=torch.float32, device=X.device) if fmt == BM_F4_E4M3 else None
-    _lib.check(L.bm_quantize_f4(X.data_ptr(), _ELEMENT[X.dtype], q.data_ptr(), s.data_ptr(), None if r is None else r.data_ptr(),
-                                R, K, ldx, fmt, scale_layout, _stream()), "bm_quantize_f4")
+    values, scales = _f4_bytes(R, K, fmt, scale_layout)
+    q = _new(X, (R, values // R), torch.uint8)
+    s = _new(X, (R, scales // R) if scale_layout == BM_SCALE_ROWS else (scales,), torch.uint8)
+    r = _new(X, (R,), torch.float32) if fmt == BM_F4_E4M3 else None
+    _lib.check(_lib.load().bm_quantize_f4(X.data_ptr(), _ELEMENT[X.dtype], q.data_ptr(), s.data_ptr(), None if r is None else r.data_ptr(),
+                                          R, K, ldx, fmt, scale_layout, _stream()), "bm_quantize_f4")
     return q, s, r
 
 
 def dequantize_f4(q, s, r, R, K, dtype=torch.float16, fmt=BM_F4_E4M3, scale_layout=BM_SCALE_TILED, out=None):
     """The numbers of a 4-bit matrix as [R, K] fp16, bf16 or fp32."""
+    parts = _f4_matrix(q, s, r, R, K, fmt, scale_layout, "Q", _device())
     if out is None:
-        out = torch.empty((R, K), dtype=dtype, device=q.device)
+        if dtype not in _ELEMENT:
+            raise BmError(f"the output cannot have dtype {dtype}")
+        out = _new(q, (R, K), dtype)
     elif _here(out, "out").dtype not in _ELEMENT or tuple(out.shape) != (R, K):
         raise BmError(f"out must be a floating-point matrix [{R}, {K}]")
-    if out.dtype not in _ELEMENT:
-        raise BmError(f"the output cannot have dtype {out.dtype}")
-    rc = _lib.load().bm_dequantize_f4(*_f4_matrix(q, s, r, R, K, fmt, scale_layout, "Q"), out.data_ptr(), _ELEMENT[out.dtype], R, K,
+    rc = _lib.load().bm_dequantize_f4(*parts, out.data_ptr(), _ELEMENT[out.dtype], R, K,
                                       _f4_rows(out, "out"), fmt, scale_layout, _stream())
     _lib.check(rc, "bm_dequantize_f4")
     return out
@@ -372,11 +399,17 @@ def f4_linear(Xq, Xs, Xr, Wq, Ws, Wr, D, M, N, K, fmt=BM_F4_E4M3):
     """D[M,N] = X W^T of two 4-bit matrices with tiled scales (X[M,K], W[N,K]; row factors may be None); D fp16, bf16 or fp32."""
     if _here(D, "D").dtype not in _ELEMENT or tuple(D.shape) != (M, N):
         raise BmError(f"D must be a floating-point matrix [{M}, {N}]")
-    x = _f4_matrix(Xq, Xs, Xr, M, K, fmt, BM_SCALE_TILED, "X")
-    w = _f4_matrix(Wq, Ws, Wr, N, K, fmt, BM_SCALE_TILED, "W")
+    device = _device()
+    x = _f4_matrix(Xq, Xs, Xr, M, K, fmt, BM_SCALE_TILED, "X", device)
+    w = _f4_matrix(Wq, Ws, Wr, N, K, fmt, BM_SCALE_TILED, "W", device)
     rc = _lib.load().bm_f4_gemm(*x, *w, D.data_ptr(), _ELEMENT[D.dtype], M, N, K, _f4_rows(D, "D"), fmt, _stream())
     _lib.check(rc, "bm_f4_gemm")
     return D
+
+
+@functools.lru_cache(maxsize=1024)
+def _moe_f4_bytes(T, H, inter, E, top):
+    return _lib.load().bm_moe_f4_workspace_bytes(T, H, inter, E, top)
 
 
 def moe_f4(X, router, w13, w2, top, inter, fmt=BM_F4_E4M3, normalize=True, out=None, workspace=None):
@@ -394,21 +427,21 @@ def moe_f4(X, router, w13, w2, top, inter, fmt=BM_F4_E4M3, normalize=True, out=N
     if router.dim() != 2 or router.shape[1] != H:
         raise BmError(f"router must be a matrix [experts, {H}]")
     E = router.shape[0]
-    router_ptr = _buffer(router, X.dtype, E * H, "router")
-    a13 = _f4_matrix(*w13, E * 2 * inter, H, fmt, BM_SCALE_ROWS, "w13")
-    a2 = _f4_matrix(*w2, E * H, inter, fmt, BM_SCALE_ROWS, "w2")
+    device = _device()
+    router_ptr = _buffer(router, X.dtype, E * H, "router", device)
+    a13 = _f4_matrix(*w13, E * 2 * inter, H, fmt, BM_SCALE_ROWS, "w13", device)
+    a2 = _f4_matrix(*w2, E * H, inter, fmt, BM_SCALE_ROWS, "w2", device)
     if out is None:
-        out = torch.empty((T, H), dtype=X.dtype, device=X.device)
+        out = _new(X, (T, H), X.dtype)
     elif _here(out, "out").dtype != X.dtype or tuple(out.shape) != (T, H):
         raise BmError(f"out must be a {X.dtype} matrix [{T}, {H}]")
-    ids = torch.empty((T, top), dtype=torch.int32, device=X.device)
-    weights = torch.empty((T, top), dtype=torch.float32, device=X.device)
-    need = L.bm_moe_f4_workspace_bytes(T, H, inter, E, top)
+    ids, weights = _new(X, (T, top), torch.int32), _new(X, (T, top), torch.float32)
+    need = _moe_f4_bytes(T, H, inter, E, top)
     if workspace is None:
-        workspace = torch.empty(max(need, 256), dtype=torch.uint8, device=X.device)
+        workspace = _new(X, (max(need, 256),), torch.uint8)
     rc = L.bm_moe_f4(X.data_ptr(), router_ptr, _ELEMENT[X.dtype], *a13, *a2, out.data_ptr(), ids.data_ptr(), weights.data_ptr(),
                      T, H, inter, E, top, ldx, _f4_rows(out, "out"), fmt, int(bool(normalize)),
-                     _buffer(workspace, torch.uint8, need, "workspace"), workspace.numel(), _stream())
+                     _buffer(workspace, torch.uint8, need, "workspace", device), workspace.numel(), _stream())
     _lib.check(rc, "bm_moe_f4")
     return out, ids, weights
 
