@@ -160,7 +160,9 @@ static int f4_few(const F4Operands& o, const F4GemmParams& g, DeviceState* dev, 
     while (p.tmem_cols < p.tokens_padded + 2 * f4_stage_tiles(o.fmt) * 4) p.tmem_cols *= 2;
     const int tiles = ceil_div(o.N, 128);
     p.split = 1;
-    while (p.split < 8 && 2 * p.split * tiles <= 2 * dev->sm_count && 2 * p.split <= p.k_blocks) p.split *= 2;
+    // Parts of K: as many as leave one CTA per SM (a second one per SM gained nothing: 16 tokens on 4096 x 4096 4.7 -> 5.3 us, on
+    // 12288 x 4096 6.7 -> 7.9, on 4096 x 11008 6.4 -> 6.4; fewer parts: 4096 x 4096 6.7 with 2 instead of 4).
+    while (p.split < kF4FewMaxSplit && 2 * p.split * tiles <= dev->sm_count && 2 * p.split <= p.k_blocks) p.split *= 2;
     CUtensorMap mw, msw, mx, msx;
     const int pitch = f4_row_bytes(o.K);
     if (int rc = make_tensor_map_u8(&mw, o.b, pitch, o.N, pitch, 128, 128, true)) return rc;
@@ -172,6 +174,28 @@ static int f4_few(const F4Operands& o, const F4GemmParams& g, DeviceState* dev, 
     BM_F4_CASE(FMT_E4M3, TYPE_F16); BM_F4_CASE(FMT_E4M3, TYPE_BF16); BM_F4_CASE(FMT_E4M3, TYPE_F32);
 #undef BM_F4_CASE
     return fail_msg(BM_ERR_LAYOUT, "unknown element type tag");
+}
+
+// Which kernel (1 few tokens, 2 tiles of 128 x 128, 3 CTA pairs).  Microseconds, fitted to 1 to 2048 tokens on weights from 1024 x 1024 to
+// 28672 x 8192 (E4M3, fp16 out): start-up plus waves, each a fixed part (the drain) and 256-wide blocks of K; half a wave where the pair
+// kernel cuts its last one.
+static int f4_choose(int M, int N, int K, int sms) {
+    const float kb = static_cast<float>(ceil_div(K, kF4BK));
+    const long long lone_tiles = static_cast<long long>(ceil_div(M, 128)) * ceil_div(N, 128);
+    const long long pair_tiles = static_cast<long long>(ceil_div(M, 256)) * ceil_div(N, 256), pairs = sms / 2;
+    const float lone = 2.6f + static_cast<float>((lone_tiles + sms - 1) / sms) * (0.55f + 0.23f * kb);
+    float pair = 1e30f;
+    if (pairs > 0) {
+        const long long rest = pair_tiles % pairs;
+        const float waves = static_cast<float>(pair_tiles / pairs) + (rest == 0 ? 0.f : pair_tiles > pairs && 2 * rest <= pairs ? 0.6f : 1.f);
+        pair = 3.0f + waves * (2.7f + 0.28f * kb);
+    }
+    // Few tokens: always up to 32, beyond while the tokens' columns cost less than the wide tiles, which stream the weights at 4 TB/s.
+    // Few-token kernel against 128 x 128: 4096 x 4096, 16 tokens 4.6 and 6.3 us, 64 tokens 7.4 and 6.4; 11008 x 4096, 48 tokens 8.3
+    // and 10.6, 64 tokens 9.0 and 7.0; 28672 x 8192, 64 tokens 25.8 and 29.2.
+    const float weight_mb = 0.5625e-6f * static_cast<float>(N) * static_cast<float>(K), stream = 2.6f + weight_mb / 4.0f;
+    if (M <= 32 || (M <= kF4FewMaxTokens && 2.3f + weight_mb / 6.4f + 0.055f * M < (lone > stream ? lone : stream))) return 1;
+    return pair < lone ? 3 : 2;
 }
 
 // ---- expert layer -----------------------------------------------------------------------
@@ -335,11 +359,11 @@ int bm_f4_gemm(const uint8_t* A, const uint8_t* SA, const float* ra, const uint8
     p.row_scale = ra;
     p.col_scale = rw;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const int forced = opt(OPT_F4_KERNEL);
-    if (M <= kF4FewMaxTokens && (forced == 1 || (forced == 0 && M <= 64))) return f4_few(o, p, dev, st);
-    const long long pair_tiles = static_cast<long long>(ceil_div(M, 256)) * ceil_div(N, 256);
-    const bool pair = dev->sm_count >= 2 && (forced == 3 || (forced != 2 && pair_tiles > dev->sm_count / 4));
-    return pair ? launch_f4<true>(o, p, dev, st) : launch_f4<false>(o, p, dev, st);
+    int kernel = opt(OPT_F4_KERNEL);
+    if (kernel == 1 && M > kF4FewMaxTokens) kernel = 0;
+    if (kernel == 0) kernel = f4_choose(M, N, K, dev->sm_count);
+    if (kernel == 1) return f4_few(o, p, dev, st);
+    return kernel == 3 && dev->sm_count >= 2 ? launch_f4<true>(o, p, dev, st) : launch_f4<false>(o, p, dev, st);
 }
 
 size_t bm_moe_f4_workspace_bytes(int T, int H, int I, int E, int top) {

@@ -15,6 +15,7 @@ namespace bm {
 constexpr int kF4FewMaxTokens = 128;
 constexpr int kF4FewThreads = 192;                        // producer, MMA issuer, 4 epilogue warps
 constexpr int kF4FewMaxStages = 8;
+constexpr int kF4FewMaxSplit = 8;
 constexpr int kF4FewRingBytes = 104 * 1024;
 constexpr int kF4FewBarOffset = kF4FewRingBytes;
 constexpr int kF4FewSmemBytes = kF4FewBarOffset + (2 * kF4FewMaxStages + 2) * 8 + 16 + 1024;
@@ -168,18 +169,22 @@ f4_gemm_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
             for (int t0 = 0; t0 < p.tokens; t0 += 16) {
                 uint32_t r[16];
                 tmem_ld_32x16(taddr + t0, r);
+                const int left = p.tokens - t0;
+                const float mine_s = p.split == 1 && p.token_scale && (lane & 15) < left ? __ldg(p.token_scale + t0 + (lane & 15)) : 1.f;
                 tmem_ld_wait();
                 if (p.split > 1) {
 #pragma unroll
                     for (int j = 0; j < 16; ++j) part[(t0 + j) * 128] = __uint_as_float(r[j]);
-                } else if (channel < p.channels) {
+                } else {
+                    float v[16];                            // all products first, then the stores
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        const int t = t0 + j;
-                        if (t < p.tokens) {
-                            const float token_s = p.token_scale ? __ldg(p.token_scale + t) : 1.f;
-                            f4_store_one<TYPE>(p.out, t * p.ld + channel, __fmul_rn(__uint_as_float(r[j]), __fmul_rn(token_s, channel_s)));
-                        }
+                    for (int j = 0; j < 16; ++j)
+                        v[j] = __fmul_rn(__uint_as_float(r[j]), __fmul_rn(__shfl_sync(0xFFFFFFFFu, mine_s, j), channel_s));
+                    if (channel < p.channels) {
+                        long long at = t0 * p.ld + channel;
+#pragma unroll
+                        for (int j = 0; j < 16; ++j, at += p.ld)
+                            if (j < left) f4_store_one<TYPE>(p.out, at, v[j]);
                     }
                 }
             }
@@ -192,11 +197,26 @@ f4_gemm_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         cluster_wait();
         if (drains && ok && channel < p.channels) {
             const uint32_t mine = smem_base + static_cast<uint32_t>(quarter * 32 + lane) * 4u;
-            for (int t = rank; t < p.tokens; t += p.split) {
-                float sum = 0.f;
-                for (int r = 0; r < p.split; ++r) sum += ld_shared_cluster_f32(mapa_shared(mine + t * 512u, r));
-                const float token_s = p.token_scale ? __ldg(p.token_scale + t) : 1.f;
-                f4_store_one<TYPE>(p.out, t * p.ld + channel, __fmul_rn(sum, __fmul_rn(token_s, channel_s)));
+            constexpr int kTogether = 4;                     // tokens whose sums are on their way together: a remote load takes 0.3 us
+            for (int t0 = rank; t0 < p.tokens; t0 += kTogether * p.split) {
+                float part[kTogether][kF4FewMaxSplit];
+#pragma unroll
+                for (int i = 0; i < kTogether; ++i)
+#pragma unroll
+                    for (int r = 0; r < kF4FewMaxSplit; ++r) {
+                        const int t = t0 + i * p.split;
+                        part[i][r] = r < p.split && t < p.tokens ? ld_shared_cluster_f32(mapa_shared(mine + t * 512u, r)) : 0.f;
+                    }
+#pragma unroll
+                for (int i = 0; i < kTogether; ++i) {
+                    const int t = t0 + i * p.split;
+                    if (t >= p.tokens) break;
+                    float sum = part[i][0];
+#pragma unroll
+                    for (int r = 1; r < kF4FewMaxSplit; ++r) sum += part[i][r];
+                    const float token_s = p.token_scale ? __ldg(p.token_scale + t) : 1.f;
+                    f4_store_one<TYPE>(p.out, t * p.ld + channel, __fmul_rn(sum, __fmul_rn(token_s, channel_s)));
+                }
             }
         }
         __syncwarp();
