@@ -815,8 +815,6 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_con
                                 b[t * 4 + c] = t < KT && c < groups && c * 4 + token < n
                                                    ? *reinterpret_cast<const uint32_t*>(tile_scales + (c * 4 + token) * scale_pitch + (kb * KT + t) * 32 + part * 4)
                                                    : 0u;
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(bar_of(sh.scale_empty[stage]));
                         if (!warp_bounded_wait(bar_of(sh.sf_empty[buf]), buf_phase ^ 1u, abort_flag, p.status, DEV_TIMEOUT_MMA_ACC_EMPTY)) { ok = false; break; }
                         tc_fence_after_sync();
                         tmem_st_32x16(tmem_base + lanes + kMoeSfBase + buf * 32, a);
@@ -824,7 +822,10 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_con
                         tmem_st_wait();
                         tc_fence_before_sync();
                         __syncwarp();
-                        if (lane == 0) mbar_arrive(bar_of(sh.sf_full[buf]));
+                        if (lane == 0) {
+                            mbar_arrive(bar_of(sh.sf_full[buf]));
+                            mbar_arrive(bar_of(sh.scale_empty[stage]));       // what was read has been used
+                        }
                         if (++stage == kMoeScaleStages) { stage = 0; phase ^= 1u; }
                         if (++buf == kMoeSfBufs) { buf = 0; buf_phase ^= 1u; }
                     }

@@ -211,3 +211,41 @@ def test_the_same_bits_on_every_call_on_streams_and_in_a_graph():
     torch.cuda.synchronize()
     layer.check(*held)
     assert_clean_status()
+
+
+@pytest.mark.parametrize("fmt", list(FMT))
+def test_a_busy_layer_gives_the_same_bits_and_the_right_ones(fmt):
+    """Every CTA has many units in a row, experts in two passes, calls follow one another without a pause."""
+    T, H, I, E, top = 32, 4096, 1408, 16, 6
+    layer = Layer(T, H, I, E, top, torch.bfloat16, FMT[fmt], seed=11)
+    x = layer.x.to(dev())
+    outs = [layer.run(x) for _ in range(40)]
+    torch.cuda.synchronize()
+    assert_clean_status()
+    assert all(torch.equal(a, b) for o in outs for a, b in zip(outs[0], o))
+    y, ids, weights = outs[0]
+    assert np.array_equal(ids.cpu().numpy(), layer.select()[1])
+    # the bound of Layer.check, on the device and with the weights given
+    w13, w2 = (ig.dequantize_f4(*layer.w[n], r, k, torch.float32, layer.fmt, ig.BM_SCALE_ROWS) for n, r, k in
+               (("w13", E * 2 * I, H), ("w2", E * H, I)))
+    u1, u2 = (H / 16 + 32) * 2.0 ** -23, (I / 16 + 32) * 2.0 ** -23
+    left = lambda v, dv: torch.from_numpy(layer.left(v.cpu().numpy(), dv if isinstance(dv, float) else dv.cpu().numpy())).to(dev())  # noqa: E731
+    xd = x.double()
+    dx = left(xd, 0.0)
+    want, bound = torch.zeros(T, H, dtype=torch.float64, device=dev()), torch.zeros(T, H, dtype=torch.float64, device=dev())
+    for e in range(E):
+        t, k = (ids == e).nonzero(as_tuple=True)
+        if len(t) == 0:
+            continue
+        a, b = w13[e * 2 * I:(e + 1) * 2 * I].double(), w2[e * H:(e + 1) * H].double()
+        gu, du = xd[t] @ a.T, (u1 * xd[t].abs() + dx[t]) @ a.abs().T
+        g, u = gu[:, :I], gu[:, I:]
+        s = g / (1 + torch.exp(-g))
+        h = s * u
+        dh = 1.1 * du[:, :I] * (u.abs() + du[:, I:]) + s.abs() * du[:, I:] + h.abs() * (8 + g.abs()) * 2.0 ** -24
+        dh = dh + left(h, dh)
+        p = weights[t, k].double()[:, None]
+        want.index_add_(0, t, p * (h @ b.T))
+        bound.index_add_(0, t, p * ((dh + u2 * h.abs()) @ b.abs().T + 1e-6 * (h @ b.T).abs()))
+    bound = bound * 1.01 + HALF[torch.bfloat16] * (want.abs() + bound)
+    assert ((y.double() - want).abs() <= bound).all()
