@@ -393,7 +393,7 @@ struct MoeShared {
     int abort_flag;
     uint32_t tmem_slot;
     unsigned long long full[kMoeStages], empty[kMoeStages], scale_full[kMoeScaleStages], scale_empty[kMoeScaleStages], sf_full[kMoeSfBufs], sf_empty[kMoeSfBufs];
-    unsigned long long acc_full[2], acc_empty[2], tile_full[2][2], tile_empty[2][2], drain;
+    unsigned long long acc_full[2], acc_empty[2], tile_full[2][2], tile_empty[2][2], slot_full[4], drain;
 };
 constexpr int kMoeStageScaleOffset = kMoeStages * kMoeStageValues;
 constexpr int kMoeTileOffset = (kMoeStageScaleOffset + kMoeScaleStages * kMoeStageScales + 1023) / 1024 * 1024;
@@ -465,6 +465,7 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_con
             mbar_init(bar_of(sh.tile_empty[0][i]), 1);
             mbar_init(bar_of(sh.tile_empty[1][i]), 1);
         }
+        for (int i = 0; i < 4; ++i) mbar_init(bar_of(sh.slot_full[i]), 1);
         mbar_init(bar_of(sh.drain), 1);
         sh.abort_flag = 0;
         fence_mbar_init();
@@ -674,7 +675,10 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_con
                             slot_scale[lane] = sh.x_scale[t];
                         }
                         __syncwarp();
-                        if (lane == 0) mbar_expect_tx(bar, n * (value_bytes + scale_bytes));
+                        if (lane == 0) {
+                            mbar_arrive(bar_of(sh.slot_full[it & 3]));
+                            mbar_expect_tx(bar, n * (value_bytes + scale_bytes));
+                        }
                         __syncwarp();
                         if (lane < n) {
                             bulk_load(smem_u32(tile) + lane * value_bytes, p.x_values + static_cast<size_t>(t) * value_bytes, value_bytes, bar);
@@ -762,6 +766,10 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_con
                     moe_row_factor<FMT>(sh.slot_top[run & 1][tid], factor, inv);
                     slot_scale[tid] = factor;
                 }
+                if (warp == kMoeFirstBuilder) {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bar_of(sh.slot_full[it & 3]));
+                }
 #pragma unroll 1
                 for (int at = warp - kMoeFirstBuilder; at < tasks; at += kMoeBuilderWarps) {
                     const int j = at / items[1], kb = at - j * items[1];
@@ -785,7 +793,10 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_con
                 ok = __all_sync(0xFFFFFFFFu, ok && *abort_flag == 0);
                 continue;
             }
-            ok = ok && warp_bounded_wait(bar_of(sh.tile_full[ph][tile_at]), tile_use & 1, abort_flag, p.status, DEV_TIMEOUT_MMA_FULL);
+            // The epilogue may be three runs behind the builders (two sums wait for it), so it has a barrier per slot of the four: a tile's
+            // barrier could have moved on by two uses.  The scale warps are never behind: an element's MMAs need their part of it.
+            ok = ok && (scales_role ? warp_bounded_wait(bar_of(sh.tile_full[ph][tile_at]), tile_use & 1, abort_flag, p.status, DEV_TIMEOUT_MMA_FULL)
+                                    : warp_bounded_wait(bar_of(sh.slot_full[it & 3]), (it >> 2) & 1, abort_flag, p.status, DEV_TIMEOUT_MMA_FULL));
             if (!ok) continue;
             const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
             if (scales_role) {

@@ -249,3 +249,16 @@ def test_a_busy_layer_gives_the_same_bits_and_the_right_ones(fmt):
         bound.index_add_(0, t, p * ((dh + u2 * h.abs()) @ b.abs().T + 1e-6 * (h @ b.T).abs()))
     bound = bound * 1.01 + HALF[torch.bfloat16] * (want.abs() + bound)
     assert ((y.double() - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("T,H,I,E,top", [(64, 16384, 64, 16, 16), (64, 64, 16384, 16, 16), (64, 256, 64, 256, 16)])
+def test_runs_of_one_unit(T, H, I, E, top):
+    """Units so short that the sums wait while the next experts' activations are made ready."""
+    layer = Layer(T, H, I, E, top, torch.bfloat16, ig.BM_F4_E8M0, seed=12)
+    x = layer.x.to(dev())
+    outs = [layer.run(x) for _ in range(10)]
+    torch.cuda.synchronize()
+    assert_clean_status()
+    assert all(torch.equal(a, b) for o in outs for a, b in zip(outs[0], o))
+    if E == 256:
+        layer.check(*outs[0])
