@@ -7,10 +7,13 @@
 
 namespace bm {
 
-static inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
+static inline int ceil_div(int a, int b) { return a / b + (a % b != 0 ? 1 : 0); }     // a + b may pass 2^31
 static inline int f4_row_bytes(int k) { return ceil_div(k, 32) * 16; }
 static inline int f4_tiles_k(int k, int fmt) { return ceil_div(k, 4 * f4_block(fmt)); }
 static inline int f4_scale_pitch(int k, int fmt) { return ceil_div(ceil_div(k, f4_block(fmt)), 16) * 16; }
+
+// indexes of 32 bits go as far as the end of a matrix's last tile: whole 256s of rows, a CTA's pieces of a row
+constexpr int kF4MaxRows = 0x7FFFFF00, kF4MaxK = 0x7FFF0000;
 
 static int check_format(int format, int layout) {
     if (format != BM_F4_E8M0 && format != BM_F4_E4M3) return fail_msg(BM_ERR_LAYOUT, "unknown 4-bit format tag");
@@ -280,7 +283,7 @@ int bm_quantize_f4(const void* X, int x_type, uint8_t* Q, uint8_t* S, float* row
     if (int rc = check_format(format, scale_layout)) return rc;
     if (x_type != BM_F16 && x_type != BM_BF16) return fail_msg(BM_ERR_LAYOUT, "X must be fp16 or bf16");
     if (format == BM_F4_E4M3 && !row_scale) return fail_msg(BM_ERR_NULL, "the E4M3 format needs row_scale");
-    if (R <= 0 || K <= 0 || K > 0x7FFFFC00 || R > 0x7FFFFF00) return fail_msg(BM_ERR_SHAPE, "R and K must be positive and below 2^31 - 1024");
+    if (R <= 0 || K <= 0 || K > kF4MaxK || R > kF4MaxRows) return fail_msg(BM_ERR_SHAPE, "R and K must be positive, at most 2^31 - 256 and 2^31 - 65536");
     if (ldx < K) return fail_msg(BM_ERR_SHAPE, "row pitch is smaller than the row length");
     if (!aligned16(Q) || !aligned16(S) || !aligned_to(X, 2) || !aligned_to(row_scale, 4))
         return fail_msg(BM_ERR_ALIGN, "Q and S must be 16-byte aligned, X and row_scale to their elements");
@@ -316,7 +319,7 @@ int bm_dequantize_f4(const uint8_t* Q, const uint8_t* S, const float* row_scale,
     if (!Q || !S || !out) return fail_msg(BM_ERR_NULL, "pointer is NULL");
     if (int rc = check_format(format, scale_layout)) return rc;
     if (out_type != BM_F16 && out_type != BM_BF16 && out_type != BM_F32) return fail_msg(BM_ERR_LAYOUT, "unknown element type tag");
-    if (R <= 0 || K <= 0 || K > 0x7FFFFC00 || R > 0x7FFFFF00) return fail_msg(BM_ERR_SHAPE, "R and K must be positive and below 2^31 - 1024");
+    if (R <= 0 || K <= 0 || K > kF4MaxK || R > kF4MaxRows) return fail_msg(BM_ERR_SHAPE, "R and K must be positive, at most 2^31 - 256 and 2^31 - 65536");
     if (ldo < K) return fail_msg(BM_ERR_SHAPE, "row pitch is smaller than the row length");
     const size_t elem = out_type == BM_F32 ? 4 : 2;
     if (!aligned16(Q) || !aligned16(S) || !aligned_to(out, elem) || !aligned_to(row_scale, 4))
@@ -342,8 +345,8 @@ int bm_f4_gemm(const uint8_t* A, const uint8_t* SA, const float* ra, const uint8
     if (!A || !SA || !W || !SW || !D) return fail_msg(BM_ERR_NULL, "pointer is NULL");
     if (int rc = check_format(format, BM_SCALE_TILED)) return rc;
     if (d_type != BM_F16 && d_type != BM_BF16 && d_type != BM_F32) return fail_msg(BM_ERR_LAYOUT, "unknown element type tag");
-    if (M <= 0 || N <= 0 || K <= 0 || K > 0x7FFFFC00 || M > 0x7FFFFF00 || N > 0x7FFFFF00)
-        return fail_msg(BM_ERR_SHAPE, "M, N, K must be positive and below 2^31 - 1024");
+    if (M <= 0 || N <= 0 || K <= 0 || K > kF4MaxK || M > kF4MaxRows || N > kF4MaxRows)
+        return fail_msg(BM_ERR_SHAPE, "M, N, K must be positive, at most 2^31 - 256 (K: 2^31 - 65536)");
     if (ldd < N) return fail_msg(BM_ERR_SHAPE, "output pitch is smaller than the row length");
     if (!aligned16(A) || !aligned16(SA) || !aligned16(W) || !aligned16(SW)) return fail_msg(BM_ERR_ALIGN, "operands and scales must be 16-byte aligned");
     if (!aligned_to(D, d_type == BM_F32 ? 4 : 2) || !aligned_to(ra, 4) || !aligned_to(rw, 4))

@@ -215,7 +215,7 @@ struct F4DequantParams {
     int vec_bytes;               // the output allows stores of 16, 8, 4 or 2 bytes
 };
 
-// out = value * scale * row factor, rounded once.  A thread per 8 columns and every fourth row of its CTA's: 4 bytes of codes, its block's scale,
+// out = value * scale * row factor in fp32, then rounded (once, if the factor is a power of two).  A thread per 8 columns and every fourth row of its CTA's: 4 bytes of codes, its block's scale,
 // 16 or 32 bytes out, four rows' loads in flight.  grid: (columns, rows)
 constexpr int kF4DequantRows = 4;
 template <int FMT, int TYPE>
@@ -224,12 +224,13 @@ dequantize_f4_kernel(const F4DequantParams p) {
     const int v = blockIdx.x * blockDim.x + threadIdx.x, k0 = v * 8;
     if (k0 >= p.k) return;
     const int g = k0 / f4_block(FMT);
-    for (int row0 = (blockIdx.y * blockDim.y + threadIdx.y) * kF4DequantRows; row0 < p.rows; row0 += gridDim.y * blockDim.y * kF4DequantRows) {
+    const unsigned rows = p.rows;                                        // (a step behind the last row may pass 2^31)
+    for (unsigned row0 = (blockIdx.y * blockDim.y + threadIdx.y) * kF4DequantRows; row0 < rows; row0 += gridDim.y * blockDim.y * kF4DequantRows) {
         uint32_t codes[kF4DequantRows], byte[kF4DequantRows];
         float t[kF4DequantRows];
 #pragma unroll
         for (int i = 0; i < kF4DequantRows; ++i) {
-            const int row = min(row0 + i, p.rows - 1);
+            const unsigned row = min(row0 + i, rows - 1);
             codes[i] = __ldg(reinterpret_cast<const uint32_t*>(p.q + static_cast<size_t>(row) * (p.k_padded / 2) + v * 4));
             byte[i] = __ldg(p.s + (p.tiles_k ? (static_cast<size_t>(row >> 7) * p.tiles_k + (g >> 2)) * kF4TileBytes + (row & 31) * 16 + ((row >> 5) & 3) * 4 + (g & 3)
                                              : static_cast<size_t>(row) * p.scale_pitch + g));
@@ -237,8 +238,8 @@ dequantize_f4_kernel(const F4DequantParams p) {
         }
 #pragma unroll
         for (int i = 0; i < kF4DequantRows; ++i) {
-            const int row = row0 + i;
-            if (row >= p.rows) break;
+            const unsigned row = row0 + i;
+            if (row >= rows) break;
             const float s = f4_scale_value<FMT>(byte[i]);
             uint32_t h[4];
             e2m1x8_to_half(codes[i], h);

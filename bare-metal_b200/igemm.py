@@ -344,7 +344,9 @@ def _f4_rows(t: torch.Tensor, name: str) -> int:
 def _f4_bytes(R, K, fmt, layout):
     """Bytes of the values and of the scales of an R x K matrix."""
     L = _lib.load()
-    values, scales = L.bm_f4_value_bytes(R, K), L.bm_f4_scale_bytes(R, K, fmt, layout)
+    values = scales = 0
+    if 0 < R < 2 ** 31 and 0 < K < 2 ** 31:              # what the entry points' arguments hold
+        values, scales = L.bm_f4_value_bytes(R, K), L.bm_f4_scale_bytes(R, K, fmt, layout)
     if not values or not scales:
         raise BmError(f"no 4-bit matrix has {R} x {K} elements, format tag {fmt} and scale layout tag {layout}")
     return values, scales

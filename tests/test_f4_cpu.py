@@ -44,6 +44,23 @@ def test_refusals():
     assert g(D=p + 1) == ALIGN and g(ra=p + 2) == ALIGN and g(t=2, D=p + 2) == ALIGN
 
 
+def test_sizes_that_do_not_fit_the_arguments():
+    """Indexes of 32 bits end before 2^31, and a size beyond an int must not come back as a small one."""
+    from bare_metal_b200 import igemm as ig
+    L = _lib.load()
+    assert L.bm_f4_value_bytes(1, 2 ** 31 - 1) == 2 ** 30 and L.bm_f4_scale_bytes(1, 2 ** 31 - 1, 1, _lib.BM_SCALE_ROWS) == 2 ** 27
+    buf = np.zeros(4096 + 64, np.uint8)
+    p = (buf.ctypes.data + 15) & ~15
+    for R, K in ((4, 2 ** 31 - 65535), (2 ** 31 - 255, 64)):
+        assert L.bm_quantize_f4(p, 0, p, p, p, R, K, K, 1, 1, None) == SHAPE
+        assert L.bm_dequantize_f4(p, p, None, p, 0, R, K, K, 1, 1, None) == SHAPE
+        assert L.bm_f4_gemm(p, p, None, p, p, None, p, 0, R, 8, K, 8, 1, None) == SHAPE
+        assert L.bm_f4_gemm(p, p, None, p, p, None, p, 0, 4, R, K, R, 1, None) == SHAPE
+    for R, K in ((2 ** 32 + 5, 64), (5, 2 ** 32 + 64), (-2 ** 32 + 5, 64), (0, 64)):
+        with pytest.raises(ig.BmError):
+            ig._f4_bytes(R, K, _lib.BM_F4_E4M3, _lib.BM_SCALE_ROWS)
+
+
 def test_expert_layer_sizes_and_refusals():
     L = _lib.load()
     assert L.bm_moe_f4_workspace_bytes(1, 64, 64, 4, 2) > 0
