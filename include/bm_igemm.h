@@ -274,10 +274,11 @@ size_t bm_f4_scale_bytes(int R, int K, int format, int scale_layout);
  *   BM_F4_E4M3  t = row_scale = 2^(floor(log2 top) - 10) (1 for a row of zeros), s = E4M3(amax / (6 t)), q = E2M1(x / (t s))
  * each rounded once to the nearest, ties to even, q saturating at 6 (exponents are held within their types' range).  A block
  * with an infinity or a NaN gets the scale NaN and the values 0.  row_scale may be NULL for BM_F4_E8M0.
- * Q and S 16-byte aligned; any K, any ldx >= K. */
+ * Q and S 16-byte aligned; any ldx >= K, K up to 2^31 - 65536, R (here and below) up to 2^31 - 256. */
 int bm_quantize_f4(const void *X, int x_type, uint8_t *Q, uint8_t *S, float *row_scale, int R, int K, int64_t ldx,
                    int format, int scale_layout, void *stream);
-/* Back to numbers: out[r][k] = value * scale * row_scale[r] (row_scale NULL: 1), rounded once to `out_type`. */
+/* Back to numbers: out[r][k] = (value * scale) * row_scale[r] in fp32 (row_scale NULL: 1; exact for powers of two), then
+ * rounded to `out_type`. */
 int bm_dequantize_f4(const uint8_t *Q, const uint8_t *S, const float *row_scale, void *out, int out_type, int R, int K,
                      int64_t ldo, int format, int scale_layout, void *stream);
 
@@ -294,10 +295,13 @@ int bm_f4_gemm(const uint8_t *A, const uint8_t *SA, const float *ra, const uint8
  * X[T x H] and router[E x H] in `x_type` (BM_F16 or BM_BF16), Y[T x H] in the same type, `ldx` / `ldy` elements between
  * rows.  W13: E matrices of 2 I rows (I gate rows, then I up rows) and K = H; W2: E matrices of H rows and K = I;
  * both in `format`, one after the other, scales in BM_SCALE_ROWS; r13 [E * 2 I] and r2 [E * H]: row factors, NULL for ones.
- * ids and weights [T x top]: the selection, in descending order, may be NULL.  Sums in fp32 (logits in 64 bits); the hidden
- * activations are rounded once, to 11 bits.  At most 64 tokens, 256 experts, top 16, H and I 16384 (BM_ERR_TOO_LARGE).
+ * ids and weights [T x top]: the selection, in descending order, may be NULL.  Sums in fp32 (logits in 64 bits).  X and the hidden
+ * activations silu(gate) * up enter the products with an error of at most 2^-16.7 of the largest of their block of 32 (16)
+ * neighbours, a small part of that number's own rounding; with BM_F4_E8M0 a number above 1.7 * 2^127 (2.9e38) counts as
+ * an infinity.  An infinity or a NaN makes the outputs that it enters NaN.  Y may be X.
+ * At most 64 tokens, 256 experts, top 16, H and I 16384 (BM_ERR_TOO_LARGE).
  * `workspace` (>= bm_moe_f4_workspace_bytes, 256-byte aligned, its contents do not matter) belongs to the call until it is
- * done: calls that may overlap need one each.  Two kernels; the second is a cooperative launch of one CTA per SM. */
+ * done: calls that may overlap need one each, captured graphs too.  Two kernels; the second is a cooperative launch of one CTA per SM. */
 size_t bm_moe_f4_workspace_bytes(int T, int H, int I, int E, int top);
 int bm_moe_f4(const void *X, const void *router, int x_type, const uint8_t *W13, const uint8_t *S13, const float *r13,
               const uint8_t *W2, const uint8_t *S2, const float *r2, void *Y, int32_t *ids, float *weights, int T, int H,

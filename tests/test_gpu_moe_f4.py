@@ -11,7 +11,9 @@ pytestmark = pytest.mark.gpu
 
 FMT = {"e8m0": ig.BM_F4_E8M0, "e4m3": ig.BM_F4_E4M3}
 HALF = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
-LOST = {torch.float16: 2.0 ** -25, torch.bfloat16: 0.0}
+# below the types' range: half of fp16's smallest number; bf16's and fp32's smallest normal one (hidden activations of 2^-240 in
+# test_the_largest_activations, outputs of 2^-239: neither exists in fp32, zero is the right answer and all of it is the error)
+LOST = {torch.float16: 2.0 ** -25, torch.bfloat16: 2.0 ** -126}
 
 
 class Layer:
@@ -51,10 +53,11 @@ class Layer:
         block is at most 32 long.)  Then the sum over the choices, and the rounding to the output type."""
         logits, order, p = self.select()
         ranked = -np.sort(-logits, 1)
+        size = np.abs(logits).max(1)                              # of a token's logits: what is added up is its own row's
         if self.top < self.E:
-            assert (ranked[:, self.top - 1] - ranked[:, self.top]).min() > 1e-6 * np.abs(logits).max(), "inputs too close to a tie"
+            assert (ranked[:, self.top - 1] - ranked[:, self.top] > 1e-6 * size).all(), "inputs too close to a tie"
         assert np.array_equal(ids.cpu().numpy(), order)
-        assert np.allclose(weights.double().cpu().numpy(), p, rtol=2e-6 * (1 + np.abs(logits).max()), atol=1e-30)
+        assert np.allclose(weights.double().cpu().numpy(), p, rtol=2e-6 * (1 + size[:, None]), atol=1e-30)
         x = self.x.double().numpy()
         want, bound = np.zeros((self.T, self.H)), np.zeros((self.T, self.H))
         w13 = f4.values(*f4.quantize(self.plain["w13"].double().numpy(), self.fmt), self.fmt)[:, :self.H]
@@ -72,7 +75,7 @@ class Layer:
                 dh = dh + self.left(h[None], dh[None])[0]
                 y1, d1 = b @ h, np.abs(b) @ dh + u2 * (np.abs(b) @ np.abs(h))
                 want[t] += p[t, k] * y1
-                bound[t] += p[t, k] * (d1 + 1e-6 * (1 + np.abs(logits).max()) * np.abs(y1))
+                bound[t] += p[t, k] * (d1 + 1e-6 * (1 + size[t]) * np.abs(y1))
         bound = bound * 1.01 + HALF[self.dtype] * (np.abs(want) + bound) + LOST[self.dtype]
         got = y.double().cpu().numpy()
         assert np.all(np.abs(got - want) <= bound), float(np.max(np.abs(got - want) / bound))
@@ -262,3 +265,33 @@ def test_runs_of_one_unit(T, H, I, E, top):
     assert all(torch.equal(a, b) for o in outs for a, b in zip(outs[0], o))
     if E == 256:
         layer.check(*outs[0])
+
+
+def test_the_largest_activations():
+    """E8M0 blocks hold up to 1.7 * 2^127; a larger number's token is NaN, not a wrong number, and the others are not touched."""
+    layer = Layer(4, 96, 40, 3, 2, torch.bfloat16, ig.BM_F4_E8M0, seed=13, spread=0.0)
+    layer.plain["w13"] = (layer.plain["w13"].float() * 2.0 ** -120).bfloat16()
+    layer.w["w13"] = ig.quantize_f4(layer.plain["w13"].to(dev()), layer.fmt, ig.BM_SCALE_ROWS)
+    layer.router_here = (layer.router.float() * 2.0 ** -125).bfloat16().to(dev())
+    layer.router = layer.router_here.cpu()
+    x = layer.x.float()
+    x[1] *= 2.0 ** 126 / x[1].abs().max()
+    x[1, 7] = 1.69 * 2.0 ** 127
+    layer.x = x.bfloat16()
+    first = layer.run()
+    layer.check(*first)
+    layer.x[2, 11] = 1.75 * 2.0 ** 127
+    y, ids, weights = layer.run()
+    assert y[2].isnan().all()
+    for t in (0, 1, 3):
+        assert torch.equal(y[t], first[0][t])
+    assert_clean_status()
+
+
+def test_the_output_may_take_the_place_of_the_input():
+    layer = Layer(19, 136, 48, 6, 2, torch.float16, ig.BM_F4_E4M3, seed=14)
+    x = layer.x.to(dev())
+    out = layer.run(x, out=x)
+    assert out[0] is x
+    layer.check(*out)
+    assert_clean_status()
