@@ -30,9 +30,11 @@
 //   The gate / up sums go to the workspace in fp32; whoever needs an expert's hidden activations waits for its sums, applies
 // SiLU and cuts them into six parts.  The experts' outputs go to the workspace in fp32 and are added per token, in the order of the
 // selection, after a last wait: no atomics on sums, the same bits on every call.
-//   Measured (device, both kernels): 64 tokens on 64 experts of 4096 x 1408, top 6, E8M0, 589 MB: 139 us, 4.2 TB/s; 16 tokens, the 221 MB
-// of their experts: 64 us, 3.5 TB/s; 1 token, 59 MB: 33 us.  About 15 us of each is not streaming: the router kernel and the
-// hand-over 6, the wait between the phases for the last sums and the first activations 4, the last wait and the sum over the experts 5.
+//   Measured (device, both kernels): 64 tokens on 64 experts of 4096 x 1408, top 6, E8M0, 589 MB: 130 us, 4.5 TB/s; 16 tokens on 128 experts
+// of 2048 x 768, top 8, E4M3, 221 MB: 60 us, 3.7 TB/s; 1 token, 59 MB: 32 us.  About 15 us of each is not streaming: the router kernel and
+// the hand-over 6, the wait between the phases for the last sums and the first activations 4, the last wait and the sum over the
+// experts 5.  Beyond that it is the chain of a stage (TMA, scales to tensor memory, MMA, release), not the bytes: with the
+// loads taken out 64 tokens still took 102 us and 16 tokens 55.
 #pragma once
 #include "f4_format.cuh"
 #include "f4_gemm.cuh"
@@ -46,13 +48,13 @@ constexpr int kMoeMaxTop = 16;
 constexpr int kMoeMaxDim = 16384;
 constexpr int kMoeParts = 6;                                    // digits of an activation
 constexpr int kMoeMaxSplit = 4;                                 // pieces of K of a unit at most
-constexpr int kMoeMaxRuns = 112;
+constexpr int kMoeMaxRuns = 80;
 
 // Activations cut up: per token and 256 of K 1 KiB, 8 rows (the 6 digits) of 128 bytes in the 128-byte swizzle of an MMA operand, and the
-// scales, per token and tile of 4 blocks 8 rows (the same for 6) of 4 bytes.
+// scales, a byte per block (the digits share it), rows of whole 16 bytes.
 __host__ __device__ constexpr int moe_k_blocks(int k) { return (k + kF4BK - 1) / kF4BK; }
 __host__ __device__ constexpr int moe_value_bytes(int k) { return moe_k_blocks(k) * 1024; }
-__host__ __device__ constexpr int moe_scale_bytes(int k, int fmt) { return moe_k_blocks(k) * f4_stage_tiles(fmt) * 32; }
+__host__ __device__ constexpr int moe_scale_bytes(int k, int fmt) { return (moe_k_blocks(k) * f4_stage_tiles(fmt) * 4 + 15) / 16 * 16; }
 
 struct MoeWorkspace {            // byte offsets
     size_t counters, x_scale, ids, weights, x_values, x_scales, gu, y, bytes;
@@ -142,7 +144,6 @@ __device__ __forceinline__ void moe_cut(const float (&x)[8], int v, uint8_t* val
     for (int j = 0; j < 8; ++j) t[j] = __float_as_uint(fmaf(x[j], inv, 12582912.f + 149796.f));
     const int block = v / SHARE, chunk = (v & 31) >> 2;
     uint8_t* row = values + (v >> 5) * 1024 + (v & 3) * 4;
-    uint8_t* scale = scales + (block >> 2) * 32 + (block & 3);
     if (odd != 0.f) byte = FMT == FMT_E4M3 ? 127u : 255u;
 #pragma unroll
     for (int i = 0; i < kMoeParts; ++i) {
@@ -157,8 +158,8 @@ __device__ __forceinline__ void moe_cut(const float (&x)[8], int v, uint8_t* val
         const uint32_t neg = (~u >> 2) & 0x11111111u;
         const uint32_t codes = (((u & 0x33333333u) ^ (neg * 3u)) + neg) | (neg << 3);
         *reinterpret_cast<uint32_t*>(row + i * 128 + ((chunk ^ i) << 4)) = codes;
-        if (v % SHARE == 0) scale[i * 4] = static_cast<uint8_t>(byte);
     }
+    if (v % SHARE == 0) scales[block] = static_cast<uint8_t>(byte);
 }
 
 // Clusters of 8 CTAs: the first ones choose the experts of up to 8 tokens each, the others cut these tokens up (a CTA per token).
@@ -359,14 +360,13 @@ constexpr int kMoeBuilderWarps = 12;
 constexpr int kMoeBuilders = 32 * kMoeBuilderWarps;             // the last warps
 constexpr int kMoeFirstBuilder = 11;
 constexpr int kMoeThreads = kMoeFirstBuilder * 32 + kMoeBuilders;   // values producer, MMA issuer, 4 scale warps, 4 epilogue warps, scales producer, builders
-constexpr int kMoeStages = 4;                                   // weight values, 256 of K
-constexpr int kMoeScaleStages = 4;                              // their scales, on their way ...
-constexpr int kMoeSfBufs = 4;                                   // ... to tensor memory
+constexpr int kMoeStages = 5;                                   // weight values, 256 of K, and as many sets of scales in tensor memory
+constexpr int kMoeScaleStages = 4;                              // scales on their way there
 constexpr int kMoeTileTokens = 16;                              // tokens of a pass at most: 128 MMA columns
 constexpr int kMoeTileBytes = 128 * 1024;                       // activations of a pass: 8 tokens of 4096, 16 of 2048
-constexpr int kMoeTileScales = 17 * 1024;
+constexpr int kMoeTileScales = 2560;                            // 2 KB and 16 bytes for each of 16 tokens, or two halves of half as much
 constexpr int kMoeStageValues = 128 * 128, kMoeStageScales = 128 * 16;
-constexpr int kMoeAccStride = 128, kMoeSfBase = 256;            // tensor memory: two accumulators, four sets of scales (32 columns each)
+constexpr int kMoeAccStride = 128, kMoeSfBase = 256;            // tensor memory: two accumulators, a set of scales (32 columns) per stage
 
 // Tiles of activations: one, or two halves where a half holds 8 tokens, so that the next is made while one is multiplied.
 __host__ __device__ constexpr int moe_tiles(int k) { return 8 * moe_value_bytes(k) <= kMoeTileBytes / 2 ? 2 : 1; }
@@ -374,7 +374,7 @@ __host__ __device__ constexpr int moe_pass_tokens(int k) {       // an even numb
     const int n = kMoeTileBytes / moe_tiles(k) / moe_value_bytes(k);
     return n < kMoeTileTokens ? n / 2 * 2 : kMoeTileTokens;
 }
-__host__ __device__ constexpr int moe_tile_scale_pitch(int k, int fmt) { return moe_scale_bytes(k, fmt) + 32; }   // tokens 8 banks apart
+__host__ __device__ constexpr int moe_tile_scale_pitch(int k, int fmt) { return moe_scale_bytes(k, fmt) + 16; }   // tokens 4 banks apart
 
 // Part of a phase's work that one CTA does with one tile of activations: elements [first, last) of an expert (element = unit *
 // pieces of K + piece), tokens of one pass.
@@ -394,7 +394,7 @@ struct MoeShared {
     uint32_t slot_top[2][kMoeTileTokens];        // per run (mod 2): largest hidden activation, fp32 bits
     int abort_flag;
     uint32_t tmem_slot;
-    unsigned long long full[kMoeStages], empty[kMoeStages], scale_full[kMoeScaleStages], scale_empty[kMoeScaleStages], sf_full[kMoeSfBufs], sf_empty[kMoeSfBufs];
+    unsigned long long full[kMoeStages], empty[kMoeStages], scale_full[kMoeScaleStages], scale_empty[kMoeScaleStages];
     unsigned long long acc_full[2], acc_empty[2], tile_full[2][2], tile_empty[2][2], slot_full[4], drain;
 };
 constexpr int kMoeStageScaleOffset = kMoeStages * kMoeStageValues;
@@ -404,11 +404,21 @@ constexpr int kMoeSharedOffset = kMoeTileScaleOffset + kMoeTileScales;
 constexpr int kMoeSmemBytes = kMoeSharedOffset + static_cast<int>(sizeof(MoeShared)) + 1024;
 static_assert(kMoeSmemBytes <= 227 * 1024, "shared memory over-subscribed");
 
-__device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t (&r)[16]) {
+__device__ __forceinline__ void tmem_st_32(uint32_t taddr, const uint32_t (&r)[16]) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};"
         ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
           "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_32(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, "
+        "%18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};"
+        ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+          "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]),
+          "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]),
+          "r"(r[31]), "r"(taddr)
         : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -446,16 +456,12 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_con
     for (int e = threadIdx.x; e < p.experts; e += kMoeThreads) sh.token_mask[e] = 0ull;
     if (threadIdx.x == 0) {
         for (int i = 0; i < kMoeStages; ++i) {
-            mbar_init(bar_of(sh.full[i]), 1);
+            mbar_init(bar_of(sh.full[i]), 5);                            // the values, and each scale warp
             mbar_init(bar_of(sh.empty[i]), 1);
         }
         for (int i = 0; i < kMoeScaleStages; ++i) {
             mbar_init(bar_of(sh.scale_full[i]), 1);
             mbar_init(bar_of(sh.scale_empty[i]), 4);
-        }
-        for (int i = 0; i < kMoeSfBufs; ++i) {
-            mbar_init(bar_of(sh.sf_full[i]), 4);
-            mbar_init(bar_of(sh.sf_empty[i]), 1);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(bar_of(sh.acc_full[i]), 1);
@@ -557,6 +563,18 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_con
         return t * p.top + choice;
     };
 
+    // pieces of K: unit and range of an element
+    auto part_of = [&](int el, int ph, int split, int& unit, int& piece, int& kb0, int& kb1) {
+        unit = el;
+        piece = kb0 = 0;
+        kb1 = items[ph];
+        if (split == 1) return;                                   // (divisions are long for one thread)
+        unit = el / split;
+        piece = el - unit * split;
+        kb0 = items[ph] * piece / split;
+        kb1 = items[ph] * (piece + 1) / split;
+    };
+
     // Every role goes through the CTA's runs, their elements and these elements' stages in the same order.
     if (warp == 0 || warp == 10) {
         // ------------------------------------------------------------------ producers: the weights' values, and their scales.  The scales run
@@ -565,85 +583,83 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_con
         const uint32_t stages = is_scales ? kMoeScaleStages : kMoeStages;
         uint32_t stage = 0, phase = 0;
         bool ok = true;
+        if (elect_one())
         for (int it = 0; it < runs && ok; ++it) {
             const int ph = it >= count0, split = sh.split[ph];
             const MoeRun r = sh.runs[ph][ph ? it - count0 : it];
             const CUtensorMap* map = is_scales ? (ph ? &map_s2 : &map_s13) : (ph ? &map_w2 : &map_w13);
             for (int el = r.first; el < r.last && ok; ++el) {
-                const int unit = el / split, piece = el - unit * split;
-                const int kb1 = items[ph] * (piece + 1) / split, row = unit * (ph ? 128 : 64), outer = ph ? r.expert : 2 * r.expert;
-                for (int kb = items[ph] * piece / split; kb < kb1; ++kb) {
-                    if (!warp_bounded_wait(is_scales ? bar_of(sh.scale_empty[stage]) : bar_of(sh.empty[stage]), phase ^ 1u, abort_flag, p.status,
-                                           DEV_TIMEOUT_PRODUCER_EMPTY)) { ok = false; break; }
-                    if (elect_one()) {
-                        if (is_scales) {
-                            const uint32_t bar = bar_of(sh.scale_full[stage]);
-                            mbar_expect_tx(bar, kMoeStageScales);
-                            tma_load_3d(smem_base + kMoeStageScaleOffset + stage * kMoeStageScales, map, bar, (FMT == FMT_E4M3 ? kb : kb >> 1) * 16, row, outer);
-                        } else {
-                            const uint32_t bar = bar_of(sh.full[stage]);
-                            mbar_expect_tx(bar, kMoeStageValues);
-                            tma_load_3d(smem_base + stage * kMoeStageValues, map, bar, kb * 128, row, outer);
-                        }
+                int unit, piece, kb0, kb1;
+                part_of(el, ph, split, unit, piece, kb0, kb1);
+                const int row = unit * (ph ? 128 : 64), outer = ph ? r.expert : 2 * r.expert;
+                for (int kb = kb0; kb < kb1; ++kb) {
+                    if (!bounded_wait(is_scales ? bar_of(sh.scale_empty[stage]) : bar_of(sh.empty[stage]), phase ^ 1u, abort_flag, p.status,
+                                      DEV_TIMEOUT_PRODUCER_EMPTY)) { ok = false; break; }
+                    if (is_scales) {
+                        const uint32_t bar = bar_of(sh.scale_full[stage]);
+                        mbar_expect_tx(bar, kMoeStageScales);
+                        tma_load_3d(smem_base + kMoeStageScaleOffset + stage * kMoeStageScales, map, bar, (FMT == FMT_E4M3 ? kb : kb >> 1) * 16, row, outer);
+                    } else {
+                        const uint32_t bar = bar_of(sh.full[stage]);
+                        mbar_expect_tx(bar, kMoeStageValues);
+                        tma_load_3d(smem_base + stage * kMoeStageValues, map, bar, kb * 128, row, outer);
                     }
-                    __syncwarp();
                     if (++stage == stages) { stage = 0; phase ^= 1u; }
                 }
             }
         }
+        __syncwarp();
     } else if (warp == 1) {
         // ------------------------------------------------------------------ MMA issuer
-        uint32_t stage = 0, phase = 0, buf = 0, buf_phase = 0, acc = 0, acc_phase = 0;
-        bool ok = true;
-        for (int it = 0; it < runs && ok; ++it) {
-            const int ph = it >= count0, run = ph ? it - count0 : it, split = sh.split[ph];
-            const MoeRun r = sh.runs[ph][run];
-            const int columns = (run_tokens(r, ph) + 1) / 2 * 16;
-            const uint32_t idesc0 = make_idesc_f4<FMT>(128, columns, 0), idesc2 = make_idesc_f4<FMT>(128, columns, 2);
-            const int tile_at = run % tiles[ph], tile_use = run / tiles[ph];
-            if (!warp_bounded_wait(bar_of(sh.tile_full[ph][tile_at]), tile_use & 1, abort_flag, p.status, DEV_TIMEOUT_MMA_FULL)) { ok = false; break; }
-            for (int el = r.first; el < r.last && ok; ++el) {
-                const int unit = el / split, piece = el - unit * split;
-                const int kb0 = items[ph] * piece / split, kb1 = items[ph] * (piece + 1) / split;
-                if (!warp_bounded_wait(bar_of(sh.acc_empty[acc]), acc_phase ^ 1u, abort_flag, p.status, DEV_TIMEOUT_MMA_ACC_EMPTY)) { ok = false; break; }
-                for (int kb = kb0; kb < kb1; ++kb) {
-                    if (!warp_bounded_wait(bar_of(sh.sf_full[buf]), buf_phase, abort_flag, p.status, DEV_TIMEOUT_MMA_FULL) ||
-                        !warp_bounded_wait(bar_of(sh.full[stage]), phase, abort_flag, p.status, DEV_TIMEOUT_MMA_FULL)) { ok = false; break; }
-                    tc_fence_after_sync();
-                    if (elect_one()) {
-                        const uint32_t d = tmem_base + acc * kMoeAccStride, sfa = tmem_base + kMoeSfBase + buf * 32, sfb = sfa + 16;
-                        const uint64_t a_desc = make_smem_desc(smem_base + stage * kMoeStageValues, 0, 1024, SWIZZLE_128B_DESC);
-                        // the 8 columns of a token are one row group; the groups lie a token's activations apart
-                        const uint64_t b_desc = make_smem_desc(smem_base + kMoeTileOffset + tile_at * (kMoeTileBytes / 2) + kb * 1024, 0, items[ph] * 1024, SWIZZLE_128B_DESC);
+        // One thread does it all, and a stage's barrier counts its values and the four scale warps: as a warp with two barriers and two
+        // commits a stage it took 850 clocks each, of which the tensor core works 170 (64 tokens 139 us, now 130).
+        const uint64_t stage_desc = make_smem_desc(smem_base, 0, 1024, SWIZZLE_128B_DESC);
+        if (elect_one()) {
+            uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
+            bool ok = true;
+            for (int it = 0; it < runs && ok; ++it) {
+                const int ph = it >= count0, run = ph ? it - count0 : it, split = sh.split[ph];
+                const MoeRun r = sh.runs[ph][run];
+                const int columns = (run_tokens(r, ph) + 1) / 2 * 16;
+                const uint32_t idesc0 = make_idesc_f4<FMT>(128, columns, 0), idesc2 = make_idesc_f4<FMT>(128, columns, 2);
+                const int tile_at = run & (tiles[ph] - 1), tile_use = run >> (tiles[ph] - 1);      // (one or two tiles)
+                // the 8 columns of a token are one row group; the groups lie a token's activations apart
+                const uint64_t tile_desc = make_smem_desc(smem_base + kMoeTileOffset + tile_at * (kMoeTileBytes / 2), 0, items[ph] * 1024, SWIZZLE_128B_DESC);
+                if (!bounded_wait(bar_of(sh.tile_full[ph][tile_at]), tile_use & 1, abort_flag, p.status, DEV_TIMEOUT_MMA_FULL)) { ok = false; break; }
+                for (int el = r.first; el < r.last && ok; ++el) {
+                    int unit, piece, kb0, kb1;
+                    part_of(el, ph, split, unit, piece, kb0, kb1);
+                    if (!bounded_wait(bar_of(sh.acc_empty[acc]), acc_phase ^ 1u, abort_flag, p.status, DEV_TIMEOUT_MMA_ACC_EMPTY)) { ok = false; break; }
+                    const uint32_t d = tmem_base + acc * kMoeAccStride;
+                    for (int kb = kb0; kb < kb1; ++kb) {
+                        if (!bounded_wait(bar_of(sh.full[stage]), phase, abort_flag, p.status, DEV_TIMEOUT_MMA_FULL)) { ok = false; break; }
+                        tc_fence_after_sync();
+                        const uint32_t sfa = tmem_base + kMoeSfBase + stage * 32, sfb = sfa + 4 * KT;
+                        const uint64_t a_desc = stage_desc + stage * (kMoeStageValues >> 4), b_desc = tile_desc + kb * (1024 >> 4);
 #pragma unroll
                         for (int ks = 0; ks < 4; ++ks) {
                             const int t = ks * KT / 4;
                             mma_f4<false, FMT>(d, a_desc + ks * 2, b_desc + ks * 2, FMT == FMT_E8M0 && (ks & 1) ? idesc2 : idesc0, sfa + t * 4, sfb + t * 4,
                                                (kb != kb0 || ks != 0) ? 1u : 0u);
                         }
-                        tc_commit(bar_of(sh.empty[stage]));
-                        tc_commit(bar_of(sh.sf_empty[buf]));
+                        tc_commit(bar_of(sh.empty[stage]));       // for the next values, and for the next scales
+                        if (++stage == kMoeStages) { stage = 0; phase ^= 1u; }
                     }
-                    __syncwarp();
-                    if (++stage == kMoeStages) { stage = 0; phase ^= 1u; }
-                    if (++buf == kMoeSfBufs) { buf = 0; buf_phase ^= 1u; }
+                    if (!ok) break;
+                    tc_commit(bar_of(sh.acc_full[acc]));
+                    acc ^= 1u;
+                    if (acc == 0) acc_phase ^= 1u;
                 }
                 if (!ok) break;
-                if (elect_one()) tc_commit(bar_of(sh.acc_full[acc]));
-                __syncwarp();
-                acc ^= 1u;
-                if (acc == 0) acc_phase ^= 1u;
+                tc_commit(bar_of(sh.tile_empty[ph][tile_at]));
             }
-            if (!ok) break;
-            if (elect_one()) tc_commit(bar_of(sh.tile_empty[ph][tile_at]));
-            __syncwarp();
+            if (!ok) {
+                tc_commit(bar_of(sh.drain));
+                const uint64_t t0 = global_timer_ns();
+                while (!mbar_try_wait(bar_of(sh.drain), 0) && global_timer_ns() - t0 < 20000000ull) {}
+            }
         }
-        if (!ok) {
-            if (elect_one()) tc_commit(bar_of(sh.drain));
-            __syncwarp();
-            const uint64_t t0 = global_timer_ns();
-            while (!mbar_try_wait(bar_of(sh.drain), 0) && global_timer_ns() - t0 < 20000000ull) {}
-        }
+        __syncwarp();
     } else {
         // ------------------------------------------------------------------ scale warps, epilogue warps and builders
         const int quarter = warp & 3, tid = static_cast<int>(threadIdx.x) - 32 * kMoeFirstBuilder;
@@ -652,7 +668,7 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_con
         bool ok = true;                                           // a builder that gave up still meets the others at their barriers
         for (int it = 0; it < runs; ++it) {
             const int ph = it >= count0, run = ph ? it - count0 : it, split = sh.split[ph], k = ph ? p.inter : p.hidden;
-            const int tile_at = run % tiles[ph], tile_use = run / tiles[ph];
+            const int tile_at = run & (tiles[ph] - 1), tile_use = run >> (tiles[ph] - 1);      // (one or two tiles)
             const MoeRun r = sh.runs[ph][run];
             const int n = run_tokens(r, ph), value_bytes = moe_value_bytes(k), scale_pitch = moe_tile_scale_pitch(k, FMT);
             uint8_t* tile = tiles0 + tile_at * (kMoeTileBytes / 2);
@@ -804,49 +820,50 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_con
             if (scales_role) {
                 // rows of scales -> tensor memory: row r of an operand in lane r % 32 of column r / 32, the same in each quarter
                 const int groups = (n * 8 + 31) / 32;             // columns of 32 activations
-                const int token = lane >> 3, part = lane & 7;
+                const int token = lane >> 3;
+                const uint8_t* token_scales = tile_scales + token * scale_pitch;
                 for (int el = r.first; el < r.last && ok; ++el) {
-                    const int unit = el / split, piece = el - unit * split;
-                    const int kb1 = items[ph] * (piece + 1) / split;
-                    for (int kb = items[ph] * piece / split; kb < kb1; ++kb) {
+                    int unit, piece, kb0, kb1;
+                    part_of(el, ph, split, unit, piece, kb0, kb1);
+                    for (int kb = kb0; kb < kb1; ++kb) {
                         if (!warp_bounded_wait(bar_of(sh.scale_full[stage]), phase, abort_flag, p.status, DEV_TIMEOUT_MMA_FULL)) { ok = false; break; }
                         const uint4* rows = reinterpret_cast<const uint4*>(smem_gen + kMoeStageScaleOffset + stage * kMoeStageScales);
-                        uint32_t a[16], b[16];
+                        uint32_t set[8 * KT];                     // KT tiles of 4 columns of W's scales, then of the activations'
 #pragma unroll
                         for (int c = 0; c < 4; ++c) {
                             const uint4 s = rows[c * 32 + lane];
+                            // all columns of a token have its scales
+                            const uint8_t* from = token_scales + c * 4 * scale_pitch + kb * KT * 4;
+                            const bool some = c < groups && c * 4 + token < n;
                             if constexpr (FMT == FMT_E4M3) {
-                                a[c] = s.x; a[4 + c] = s.y; a[8 + c] = s.z; a[12 + c] = s.w;
+                                const uint4 x = some ? *reinterpret_cast<const uint4*>(from) : make_uint4(0, 0, 0, 0);
+                                set[c] = s.x; set[4 + c] = s.y; set[8 + c] = s.z; set[12 + c] = s.w;
+                                set[16 + c] = x.x; set[20 + c] = x.y; set[24 + c] = x.z; set[28 + c] = x.w;
                             } else {                              // 16 bytes are 512 of K: this stage's half of them
-                                a[c] = kb & 1 ? s.z : s.x; a[4 + c] = kb & 1 ? s.w : s.y; a[8 + c] = a[12 + c] = 0;
+                                const uint2 x = some ? *reinterpret_cast<const uint2*>(from) : make_uint2(0, 0);
+                                set[c] = kb & 1 ? s.z : s.x; set[4 + c] = kb & 1 ? s.w : s.y;
+                                set[8 + c] = x.x; set[12 + c] = x.y;
                             }
                         }
-#pragma unroll
-                        for (int t = 0; t < 4; ++t)
-#pragma unroll
-                            for (int c = 0; c < 4; ++c)
-                                b[t * 4 + c] = t < KT && c < groups && c * 4 + token < n
-                                                   ? *reinterpret_cast<const uint32_t*>(tile_scales + (c * 4 + token) * scale_pitch + (kb * KT + t) * 32 + part * 4)
-                                                   : 0u;
-                        if (!warp_bounded_wait(bar_of(sh.sf_empty[buf]), buf_phase ^ 1u, abort_flag, p.status, DEV_TIMEOUT_MMA_ACC_EMPTY)) { ok = false; break; }
+                        if (!warp_bounded_wait(bar_of(sh.empty[buf]), buf_phase ^ 1u, abort_flag, p.status, DEV_TIMEOUT_MMA_ACC_EMPTY)) { ok = false; break; }
                         tc_fence_after_sync();
-                        tmem_st_32x16(tmem_base + lanes + kMoeSfBase + buf * 32, a);
-                        tmem_st_32x16(tmem_base + lanes + kMoeSfBase + buf * 32 + 16, b);
+                        tmem_st_32(tmem_base + lanes + kMoeSfBase + buf * 32, set);
                         tmem_st_wait();
                         tc_fence_before_sync();
                         __syncwarp();
                         if (lane == 0) {
-                            mbar_arrive(bar_of(sh.sf_full[buf]));
+                            mbar_arrive(bar_of(sh.full[buf]));
                             mbar_arrive(bar_of(sh.scale_empty[stage]));       // what was read has been used
                         }
                         if (++stage == kMoeScaleStages) { stage = 0; phase ^= 1u; }
-                        if (++buf == kMoeSfBufs) { buf = 0; buf_phase ^= 1u; }
+                        if (++buf == kMoeStages) { buf = 0; buf_phase ^= 1u; }
                     }
                 }
             } else {
                 const int row = quarter * 32 + lane;              // gate / up: rows 0-63 gate, 64-127 up of 64 channels
                 for (int el = r.first; el < r.last && ok; ++el) {
-                    const int unit = el / split, piece = el - unit * split;
+                    int unit, piece, kb0, kb1;
+                    part_of(el, ph, split, unit, piece, kb0, kb1);
                     const int channel = ph ? unit * 128 + row : unit * 64 + (row & 63), limit = ph ? p.hidden : p.inter;
                     const bool in = channel < limit;
                     float factor = 1.f;
