@@ -14,7 +14,8 @@
 // 2 bytes in and 1/2 + 1/16 (1/32) out per element.  A group of threads per row holds it in registers, units of 16 numbers (a block,
 // or half of one), so the row's maximum costs no second read.  What bounds it with many rows is instructions as much as bytes: an
 // element gets one conversion, one FMA and one subtraction before the packing conversion, a unit its maximum once and its
-// scale once (8 numbers a thread and two threads a block took 171 instructions per 8).
+// scale once (8 numbers a thread and two threads a block took 171 instructions per 8, this 103).  8192 x 11008 bf16 to E4M3 46 us, 5.0 TB/s;
+// 8192 x 4096 to E8M0 15.8 us, 5.4 TB/s; 4096 x 4096 fp16 to E4M3 10.6 us.  Issue slots are 67 % busy, the rest waits for loads.
 #pragma once
 #include "f4_format.cuh"
 
