@@ -247,7 +247,10 @@ inline int cached_tensor_map(CUtensorMap* map, const void* base, int rank, CUten
     }
     std::lock_guard<std::mutex> lock(cache.mutex);
     if (cache.maps.size() >= kMapCacheCapacity) cache.maps.clear();
-    cache.maps.emplace(key, *map);
+    try {
+        cache.maps.emplace(key, *map);
+    } catch (...) {                                  // out of memory: encoded again next time; nothing may leave a C entry point
+    }
     cache.misses.fetch_add(1, std::memory_order_relaxed);
     return BM_OK;
 }
