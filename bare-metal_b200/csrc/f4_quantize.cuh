@@ -14,8 +14,8 @@
 // 2 bytes in and 1/2 + 1/16 (1/32) out per element.  A group of threads per row holds it in registers, units of 16 numbers (a block,
 // or half of one), so the row's maximum costs no second read.  What bounds it with many rows is instructions as much as bytes: an
 // element gets one conversion, one FMA and one subtraction before the packing conversion, a unit its maximum once and its
-// scale once (8 numbers a thread and two threads a block took 171 instructions per 8, this 103).  8192 x 11008 bf16 to E4M3 46 us, 5.0 TB/s;
-// 8192 x 4096 to E8M0 15.8 us, 5.4 TB/s; 4096 x 4096 fp16 to E4M3 10.6 us.  Issue slots are 67 % busy, the rest waits for loads.
+// scale once (8 numbers a thread and two threads a block took 171 instructions per 8, this 103).  8192 x 11008 bf16 to E4M3 45.1 us, 5.1 TB/s;
+// 8192 x 4096 to E8M0 15.8 us, 5.4 TB/s; 4096 x 4096 fp16 to E4M3 10.4 us.  Issue slots are 67 % busy, the rest waits for loads.
 #pragma once
 #include "f4_format.cuh"
 
@@ -130,7 +130,9 @@ __device__ __forceinline__ void f4_emit(const F4QuantParams& p, const F4RowOut& 
         const float t = __fmul_rn(a, out.inv_row), guess = __fmul_rn(t, 1.f / 6.f);
         byte = __nv_cvt_float_to_fp8(__fmaf_rn(__fmaf_rn(-6.f, guess, t), 1.f / 6.f, guess), __NV_SATFINITE, __NV_E4M3);
         const float s = e4m3_value(byte);
-        const float inv = byte != 0 ? __fmul_rn(__fdividef(1.f, s), out.inv_row) : 0.f;
+        float inv;                                                      // off by 2^-23 at most; __fdividef takes 2 % more of the kernel's time
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+        inv = byte != 0 ? __fmul_rn(inv, out.inv_row) : 0.f;
 #pragma unroll
         for (int j = 0; j < 16; ++j) f[j] = __fsub_rn(__fmaf_rn(f[j], inv, 768.f), 768.f);
         if (odd) byte = 127;
