@@ -8,12 +8,13 @@
 // The products run on tcgen05.mma.kind::mxf4nvf4, which takes the weights as they are stored; nothing is done per weight outside
 // the tensor core.  (Converting them to fp16 in registers for mma.sync took 2.2 instructions a weight and reached
 // 1.9 TB/s; the conversion instruction alone runs at 16 weights a clock and SM, a third of what HBM delivers.)  It wants
-// the activations in 4 bits too, so each is written with six digits of base 8 under its block's scale,
-//     x = s * sum over i < 6 of 8^-i * d_i / 2,   d_i from -4 to 3: all of them E2M1 numbers when halved,
-// which leaves 2^-17 s < 2^-16.7 of the block's largest, far less than fp16's own rounding of it (2^-12).  The six digits are six
-// columns of the MMA and cost nothing: an MMA takes as long with 8 columns as with 100.  All six have the block's scale;
-// the powers of 8 are applied to the columns' fp32 sums when they are added.  (Six E2M1 numbers by repeated rounding of what is left
-// are as exact and took three times the instructions.)
+// the activations in 4 bits too, so each is written with eight digits of base 8 under its block's scale,
+//     x = s * sum over i < 8 of 8^-i * d_i / 2,   d_i from -4 to 3: all of them E2M1 numbers when halved.
+// s is a power of two, so x is a multiple of 2^-22 s (an fp16 number down to 2^-12 of its block's largest) exactly, any other
+// off by at most 2^-23 s < 2^-22.7 of the block's largest: the rounding of an fp32 number.  (Six digits, 2^-16.7, were not
+// enough beside a channel a thousand times larger: 2^-7 of the others.)  The eight digits are eight columns of the MMA, the
+// least it takes, and cost nothing: an MMA takes as long with 8 columns as with 100.  All have the block's scale; the powers of 8
+// are applied to the columns' fp32 sums when they are added.
 //
 // Kernel 1, moe_router_kernel: clusters of 8 CTAs per group of at most 8 tokens.  One set of clusters makes the logits: the warps share the
 // experts and 16 pieces of K (mma.sync, 16 experts x 8 tokens), the pieces meet in the shared memory of one CTA per token, whose first
@@ -28,7 +29,7 @@
 // tensor memory by four warps (tcgen05.st) on the way.  The ring runs ahead into the next expert and, over the wait
 // for the other CTAs' gate / up sums, into the down projection's weights.
 //   The gate / up sums go to the workspace in fp32; whoever needs an expert's hidden activations waits for its sums, applies
-// SiLU and cuts them into six parts.  The experts' outputs go to the workspace in fp32 and are added per token, in the order of the
+// SiLU and cuts them into digits.  The experts' outputs go to the workspace in fp32 and are added per token, in the order of the
 // selection, after a last wait: no atomics on sums, the same bits on every call.
 //   Measured (device, both kernels): 64 tokens on 64 experts of 4096 x 1408, top 6, E8M0, 589 MB: 130 us, 4.5 TB/s; 16 tokens on 128 experts
 // of 2048 x 768, top 8, E4M3, 221 MB: 60 us, 3.7 TB/s; 1 token, 59 MB: 32 us.  About 15 us of each is not streaming: the router kernel and
@@ -46,11 +47,11 @@ constexpr int kMoeMaxTokens = 64;
 constexpr int kMoeMaxExperts = 256;
 constexpr int kMoeMaxTop = 16;
 constexpr int kMoeMaxDim = 16384;
-constexpr int kMoeParts = 6;                                    // digits of an activation
+constexpr int kMoeParts = 8;                                    // digits of an activation
 constexpr int kMoeMaxSplit = 4;                                 // pieces of K of a unit at most
 constexpr int kMoeMaxRuns = 80;
 
-// Activations cut up: per token and 256 of K 1 KiB, 8 rows (the 6 digits) of 128 bytes in the 128-byte swizzle of an MMA operand, and the
+// Activations cut up: per token and 256 of K 1 KiB, 8 rows (the digits) of 128 bytes in the 128-byte swizzle of an MMA operand, and the
 // scales, a byte per block (the digits share it), rows of whole 16 bytes.
 __host__ __device__ constexpr int moe_k_blocks(int k) { return (k + kF4BK - 1) / kF4BK; }
 __host__ __device__ constexpr int moe_value_bytes(int k) { return moe_k_blocks(k) * 1024; }
@@ -100,22 +101,23 @@ __device__ __forceinline__ uint4 moe_piece(const uint16_t* row, int v, int k, bo
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// FMT_E4M3: the power of two 2^e that puts a row's largest |v| (fp32 bits) in [2^8, 2^9), where 0.625 times it is a scale, as v / 2^e
+// FMT_E4M3: the power of two 2^e that puts a row's largest |v| (fp32 bits) in [2^7, 2^8), where its scale is at most 2^8, as v / 2^e
 template <int FMT>
 __device__ __forceinline__ void moe_row_factor(uint32_t top_bits, float& factor, float& inv) {
     factor = inv = 1.f;
     if (FMT == FMT_E8M0 || top_bits == 0 || top_bits >= 0x7F800000u) return;
-    const int lg = static_cast<int>(top_bits >> 23), e = lg > 9 ? lg - 8 : 1;
+    const int lg = static_cast<int>(top_bits >> 23), e = lg > 8 ? lg - 7 : 1;
     factor = __uint_as_float(static_cast<uint32_t>(e) << 23);
     inv = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
 }
 
 // Eight activations (piece v of a row, two or four neighbouring lanes share a block) as digits and scales.  `values`, `scales`: the
 // token's own places, in shared or global memory.  Whole warps.
-//   The scale is at least |largest| / 1.7067: six digits reach 1.714.  A number times 2^16 / s, rounded to an integer m, plus 4 in every
-// digit, are the 18 low bits of the sum with 1.5 * 2^23: one FMA, and digit + 4 are three of its bits.
+//   The scale is the smallest power of two of at least |largest| / 1.7 (eight digits reach 1.714) that the format has: 2^-126
+// (E8M0), or 2^-9 under the row's factor (E4M3: 2^-16 of the row's largest or less).  A number times 2^22 / s, rounded to an integer, plus 4 in every
+// digit, is 24 bits, three of them a digit + 4.
 template <int FMT>
-__device__ __forceinline__ void moe_cut(const float (&x)[8], int v, uint8_t* values, uint8_t* scales) {
+__device__ __forceinline__ void moe_cut(float (&x)[8], int v, uint8_t* values, uint8_t* scales) {
     constexpr int SHARE = f4_block(FMT) / 8;
     float odd = 0.f;                                              // a NaN where one of the block's numbers is none
 #pragma unroll
@@ -127,21 +129,21 @@ __device__ __forceinline__ void moe_cut(const float (&x)[8], int v, uint8_t* val
         top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
         odd += __shfl_xor_sync(0xFFFFFFFFu, odd, o);
     }
-    uint32_t byte;
-    float inv;                                                    // 2^16 / s
+    // the scale's exponent + 127; 255 for an infinity and for a number above 1.7 * 2^127, which no E8M0 scale holds
+    uint32_t e = (__float_as_uint(top * 0.58823530f) + 0x007FFFFFu) >> 23;
+    uint32_t byte = e;
     if constexpr (FMT == FMT_E4M3) {
-        // to the nearest, off by a 16th at most; half a step more where steps are even (below 2^-6), so never below there
-        byte = __nv_cvt_float_to_fp8(fmaf(top, 0.625f, 0x1p-10f), __NV_SATFINITE, __NV_E4M3);
-        inv = byte != 0 ? __fdividef(65536.f, e4m3_value(byte)) : 0.f;
-    } else {
-        // the smallest power of two that holds the largest below 1.7 (2^-110 at least: what is smaller is nothing in fp32 sums); a
-        // number above 1.7 * 2^127, the last one, makes its block NaN (255) like an infinity
-        byte = max((__float_as_uint(top * 0.58823530f) + 0x007FFFFFu) >> 23, 17u);
-        inv = __uint_as_float((254u + 16u - byte) << 23);
+        e = min(max(e, 127u - 9u), 127u + 8u);
+        byte = e >= 121u ? (e - 120u) << 3 : 1u << (e - 118u);   // a normal E4M3 number from 2^-6 on
+    } else if (e < 22u) {                                         // 2^22 / s would leave fp32's range
+        e += 64u;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] *= 0x1p64f;
     }
+    const float inv = __uint_as_float((254u + 22u - e) << 23);   // 2^22 / s
     uint32_t t[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) t[j] = __float_as_uint(fmaf(x[j], inv, 12582912.f + 149796.f));
+    for (int j = 0; j < 8; ++j) t[j] = static_cast<uint32_t>(__float2int_rn(x[j] * inv)) + 9586980u;
     const int block = v / SHARE, chunk = (v & 31) >> 2;
     uint8_t* row = values + (v >> 5) * 1024 + (v & 3) * 4;
     if (odd != 0.f) byte = FMT == FMT_E4M3 ? 127u : 255u;
