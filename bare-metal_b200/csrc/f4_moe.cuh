@@ -10,8 +10,8 @@
 // 1.9 TB/s; the conversion instruction alone runs at 16 weights a clock and SM, a third of what HBM delivers.)  It wants
 // the activations in 4 bits too, so each is written with eight digits of base 8 under its block's scale,
 //     x = s * sum over i < 8 of 8^-i * d_i / 2,   d_i from -4 to 3: all of them E2M1 numbers when halved.
-// s is a power of two, so x is a multiple of 2^-22 s (an fp16 number down to 2^-12 of its block's largest) exactly, any other
-// off by at most 2^-23 s < 2^-22.7 of the block's largest: the rounding of an fp32 number.  (Six digits, 2^-16.7, were not
+// s is a power of two, so multiples of 2^-22 s (fp16 numbers down to 2^-10 of their block's largest, bf16 down to 2^-13) are exact,
+// others off by at most 2^-23 s < 2^-22.7 of the block's largest.  (Six digits, 2^-16.7, were not
 // enough beside a channel a thousand times larger: 2^-7 of the others.)  The eight digits are eight columns of the MMA, the
 // least it takes, and cost nothing: an MMA takes as long with 8 columns as with 100.  All have the block's scale; the powers of 8
 // are applied to the columns' fp32 sums when they are added.

@@ -297,8 +297,9 @@ int bm_f4_gemm(const uint8_t *A, const uint8_t *SA, const float *ra, const uint8
  * both in `format`, one after the other, scales in BM_SCALE_ROWS; r13 [E * 2 I] and r2 [E * H]: row factors, NULL for ones.
  * ids and weights [T x top]: the selection, in descending order, may be NULL.  Sums in fp32 (logits in 64 bits).  X and the hidden
  * activations silu(gate) * up enter the products as fixed-point numbers of 24 bits under the largest of their block of 32 (16)
- * neighbours: off by at most 2^-22.7 of it (BM_F4_E4M3: or 2^-39 of their row's largest, if that is more), exact where they are fp16
- * or bf16 numbers down to 2^-12 of it (bf16: 2^-15); with BM_F4_E8M0 a number above 1.7 * 2^127 (2.9e38) counts as an infinity.  An infinity or a NaN makes the outputs that it enters NaN.  Y may be X.
+ * neighbours: off by at most 2^-22.7 of it (BM_F4_E4M3: or 2^-39 of their row's largest, if that is more), exact where they are
+ * fp16 numbers down to 2^-10 of it or bf16 numbers down to 2^-13; with BM_F4_E8M0 a number above 1.7 * 2^127 (2.9e38) counts as an
+ * infinity.  An infinity or a NaN makes the outputs that it enters NaN.  Y may be X.
  * At most 64 tokens, 256 experts, top 16, H and I 16384 (BM_ERR_TOO_LARGE).
  * `workspace` (>= bm_moe_f4_workspace_bytes, 256-byte aligned, its contents do not matter) belongs to the call until it is
  * done: calls that may overlap need one each, captured graphs too.  Two kernels; the second is a cooperative launch of one CTA per SM. */
