@@ -262,6 +262,7 @@ static int dense_gemm(int epi, const int8_t* A, const int8_t* B, void* C, int M,
         if (n_peers > kMaxOutMaps) return fail_msg(BM_ERR_TOO_LARGE, "at most 8 gather destinations");
         for (int d = 0; d < n_peers; ++d) {
             if (!peers[d] || !aligned16(peers[d])) return fail_msg(BM_ERR_ALIGN, "gather destinations must be 16-byte aligned");
+            map_out.base[d] = peers[d];
             if (int rc = make_tensor_map_out(&map_out.m[d], peers[d], N, M, static_cast<size_t>(ldc) * out_elem_size(epi),
                                              static_cast<int>(out_elem_size(epi))))
                 return rc;
@@ -280,6 +281,7 @@ static int dense_gemm(int epi, const int8_t* A, const int8_t* B, void* C, int M,
         // one remote store = one 32-row x 128-byte box = 4 KiB; virtual-clock units are 1/16 ns
         p.pace.cost = gbs > 0 ? static_cast<unsigned>((4096.0 * 16.0) / gbs + 0.5) : 0u;
     } else if (p.epi.vec_ok && opt(OPT_TMA_STORE) != 0) {
+        map_out.base[0] = C;
         if (int rc = make_tensor_map_out(&map_out.m[0], C, N, M, static_cast<size_t>(ldc) * out_elem_size(epi),
                                          static_cast<int>(out_elem_size(epi))))
             return rc;

@@ -139,27 +139,6 @@ __device__ __forceinline__ uint4 f4_convert16(const uint32_t* r, const float* co
     }
 }
 
-// A staged box (32 rows of 128 bytes, 128-byte swizzle) to the output, a row at a time: 128 bytes side by side by the 32 lanes.  (Each lane
-// storing its own row, element by element, took 33 us for 777 x 2260 x 1000 in fp16.)
-template <class T>
-__device__ __forceinline__ void f4_copy_box(const F4GemmParams& p, uint32_t stage_smem, int row0, int col0, int lane) {
-    constexpr int PER = 4 / sizeof(T);
-    const int col = col0 + lane * PER, rows = min(32, p.rows - row0);
-    T* dst = reinterpret_cast<T*>(p.out) + static_cast<long long>(row0) * p.ld + col;
-#pragma unroll 4
-    for (int r = 0; r < rows; ++r, dst += p.ld) {
-        uint32_t w;
-        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(stage_smem + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4) : "memory");
-        if (PER == 1 || p.pair_ok) {
-            if (col + PER <= p.cols) { *reinterpret_cast<uint32_t*>(dst) = w; continue; }
-        }
-        const T* t = reinterpret_cast<const T*>(&w);
-#pragma unroll
-        for (int j = 0; j < PER; ++j)
-            if (col + j < p.cols) dst[j] = t[j];
-    }
-}
-
 // Drains NC columns of 32 rows (one per lane) in chunks of 32.  `reverse`: the upper half of the chunks first (NC = 128).
 // `first_half` is called once, when the first 64 columns have left the accumulator.
 template <int TYPE, int NC, class Hook>
@@ -213,7 +192,7 @@ __device__ __forceinline__ void f4_drain(const F4GemmParams& p, const CUtensorMa
                 }
             } else {
                 __syncwarp();
-                f4_copy_box<T>(p, stage_smem, row0, box_c0, lane);
+                copy_staged_box<T, 4>(p.out, p.ld, p.rows, p.cols, p.pair_ok != 0, stage_smem, row0, box_c0, lane);
                 __syncwarp();
             }
         }

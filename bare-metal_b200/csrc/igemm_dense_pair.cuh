@@ -247,7 +247,7 @@ igemm_dense_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
                                    (narrow ? half * 64 : half * kPairNC);
             const uint32_t my_stage = smem_base + kPairStoreOffset + (warp - 2) * kPairStoreBufs * kStoreBoxBytes;
             if (p.epi.tma_ok)
-                drain_accumulator_tma<EPI, kPairNC, kPairStoreBufs>(p.epi, maps_out.m, p.n_out, taddr, row_base, lane,
+                drain_accumulator_tma<EPI, kPairNC, kPairStoreBufs>(p.epi, maps_out.m, B_MN ? nullptr : maps_out.base, p.n_out, taddr, row_base, lane,
                                                                     n0, strip, lane_s, my_stage, box_count, col_limit, p.pace);
             else
                 drain_accumulator<EPI, kPairNC, false>(p.epi, taddr, row, n0, col_limit, strip, lane_s);

@@ -309,7 +309,7 @@ igemm_sparse_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid
                                                 smem_base + PC::STORE_OFFSET + (warp - 2) * kNarrowBoxBytes, t_limit,
                                                 half == 1, overlap_read);
                     else
-                        drain_tma_from<EPI, kSpPairNC, 1>(p.epi, &map_out, 1, TmemSource{taddr}, n0 + quarter * 32, lane, t0, strip,
+                        drain_tma_from<EPI, kSpPairNC, 1>(p.epi, &map_out, nullptr, 1, TmemSource{taddr}, n0 + quarter * 32, lane, t0, strip,
                                                           lane_s, smem_base + PC::STORE_OFFSET + (warp - 2) * kStoreBoxBytes,
                                                           box_count, t_limit, StorePace{nullptr, 0u, 0u, 0}, overlap_read, half == 1);
                     stored = true;
