@@ -678,13 +678,16 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_con
             uint16_t* slot_row = sh.slot_row[it & 3];
             float* slot_scale = sh.slot_scale[it & 3];
             if (!scales_role && !epilogue_role) {
-                // the tile's last use is over (all builders keep up with every run, so a barrier is never two phases ahead)
+                // The tile's last use is over.  Only the first builder warp waits for that, and for every use in turn, so the barrier is never two
+                // phases ahead of it: no tile is filled without it.  The others, who have nothing to do for gate / up, could be any number
+                // of phases behind; they touch a tile only behind the builders' own barrier.
                 auto wait_empty = [&](int phs, int at, int parity) {
                     ok = ok && warp_bounded_wait(bar_of(sh.tile_empty[phs][at]), parity, abort_flag, p.status, DEV_TIMEOUT_PRODUCER_EMPTY);
                 };
-                wait_empty(ph, tile_at, (tile_use & 1) ^ 1);
+                if (ph == 0 && warp != kMoeFirstBuilder) continue;
+                if (warp == kMoeFirstBuilder) wait_empty(ph, tile_at, (tile_use & 1) ^ 1);
                 if (ph == 0) {
-                    if (warp == kMoeFirstBuilder && ok) {                       // copies what the router kernel has cut
+                    if (ok) {                                     // copies what the router kernel has cut
                         const uint32_t bar = bar_of(sh.tile_full[0][tile_at]);
                         const int scale_bytes = moe_scale_bytes(k, FMT);
                         int t = 0;
@@ -708,7 +711,7 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_con
                     continue;
                 }
                 // ---- hidden activations of the pass: silu(gate) * up from the sums of all CTAs, cut into their parts
-                if (run == 0)                                     // (the tiles of both phases share their memory)
+                if (run == 0 && warp == kMoeFirstBuilder)         // (the tiles of both phases share their memory)
                     for (int i = 0; i < tiles[0] && i < count0; ++i) {
                         const int last = (count0 - 1 - i) / tiles[0];     // use of the tile that run count0 - 1 - i had
                         wait_empty(0, (count0 - 1 - i) % tiles[0], last & 1);

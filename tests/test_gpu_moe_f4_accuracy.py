@@ -6,7 +6,7 @@ import torch
 import _f4 as f4
 from bare_metal_b200 import igemm as ig
 from _gpu import assert_clean_status, dev
-from test_gpu_moe_f4 import FMT, Layer
+from test_gpu_moe_f4 import FMT, HALF, LOST, Layer
 
 pytestmark = pytest.mark.gpu
 
@@ -65,3 +65,49 @@ def test_tiny_bf16_activations_under_weights_with_large_scales(scale):
     assert_clean_status()
     layer.check(*out)
     assert out[0].abs().max() > 0.01
+
+
+def check_on_device(layer, y, ids, weights):
+    """Layer.check's bound in 64 bits on the device, for layers that are too large for it, with the selection and the weights given."""
+    T, H, I, E = layer.T, layer.H, layer.I, layer.E
+    assert np.array_equal(ids.cpu().numpy(), layer.select()[1])
+    w13, w2 = (ig.dequantize_f4(*layer.w[n], r, k, torch.float32, layer.fmt, ig.BM_SCALE_ROWS) for n, r, k in (("w13", E * 2 * I, H), ("w2", E * H, I)))
+    u1, u2 = (H / 16 + 32) * 2.0 ** -23, (I / 16 + 32) * 2.0 ** -23
+    left = lambda v, dv: torch.from_numpy(layer.left(v.cpu().numpy(), dv.cpu().numpy())).to(dev())  # noqa: E731
+    x = layer.x.to(dev()).double()
+    dx = left(x, torch.zeros_like(x))
+    want, bound = torch.zeros(T, H, dtype=torch.float64, device=dev()), torch.zeros(T, H, dtype=torch.float64, device=dev())
+    for e in range(E):
+        t, k = (ids == e).nonzero(as_tuple=True)
+        if len(t) == 0:
+            continue
+        a, b = w13[e * 2 * I:(e + 1) * 2 * I].double(), w2[e * H:(e + 1) * H].double()
+        gu, du = x[t] @ a.T, (u1 * x[t].abs() + dx[t]) @ a.abs().T
+        g, u = gu[:, :I], gu[:, I:]
+        s = g / (1 + torch.exp(-g))
+        h = s * u
+        dh = 1.1 * du[:, :I] * (u.abs() + du[:, I:]) + s.abs() * du[:, I:] + h.abs() * (8 + g.abs()) * 2.0 ** -24
+        dh = dh + left(h, dh)
+        p = weights[t, k].double()[:, None]
+        want.index_add_(0, t, p * (h @ b.T))
+        bound.index_add_(0, t, p * ((dh + u2 * h.abs()) @ b.abs().T + 1e-6 * (h @ b.T).abs()))
+    bound = bound * 1.01 + HALF[layer.dtype] * (want.abs() + bound) + LOST[layer.dtype]
+    assert ((y.double() - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("fmt", list(FMT))
+@pytest.mark.parametrize("T,H,I,E,top", [(64, 16384, 64, 16, 16), (64, 64, 16384, 16, 16), (64, 2304, 64, 64, 16), (48, 2048, 80, 200, 16)])
+def test_many_short_runs_beside_a_busy_stream(T, H, I, E, top, fmt):
+    """Tiles of activations that change hands after every unit of work, while other kernels take their share of the SMs."""
+    layer = FineLayer(T, H, I, E, top, torch.bfloat16, FMT[fmt], seed=31)
+    x = layer.x.to(dev())
+    first = layer.run(x)
+    torch.cuda.synchronize()
+    check_on_device(layer, *first)
+    side, noise = torch.cuda.Stream(), torch.zeros(1 << 24, device=dev())
+    for _ in range(12):
+        with torch.cuda.stream(side):
+            noise.add_(1.0)
+        again = layer.run(x)
+        assert all(torch.equal(a, b) for a, b in zip(first, again))
+    assert_clean_status()
