@@ -19,8 +19,9 @@
 // Kernel 1, moe_router_kernel: clusters of 8 CTAs per group of at most 8 tokens.  One set of clusters makes the logits: the warps share the
 // experts and 16 pieces of K (mma.sync, 16 experts x 8 tokens), the pieces meet in the shared memory of one CTA per token, whose first
 // warp selects.  Another set of clusters cuts the same tokens into their digits meanwhile, a CTA per token.
-// Logits are added in fp32 over 16 products and in 64 bits beyond, in a fixed order: which expert a token gets must not depend on
-// the batch the token is in.
+// Logits are products and sums in 64 bits (mma.sync on fp64), in an order that is the same for every token of every batch.  With sums
+// of 16 products in fp32 the kernel was 1.6 us shorter, but logits that large channels cancel in were ordered wrongly, equal ones
+// told apart, and products of bf16 beyond 2^128 made infinities of finite logits.
 //
 // Kernel 2, moe_experts_kernel: one CTA per SM, all resident (cooperative launch).  The unit of work is 128 weight rows (gate / up: 64
 // channels of each) times the tokens of one expert; where units are few they are cut along K, and the parts' sums are
@@ -168,21 +169,23 @@ __device__ __forceinline__ void moe_cut(float (&x)[8], int v, uint8_t* values, u
 constexpr int kMoeRouterCtas = 8, kMoeRouterThreads = 256, kMoeRouterTokens = 8;
 constexpr int kMoeRouterChunks = 16;                             // pieces of K that the logits are added up from
 
+// D = A B + C in 64 bits: A 16 x 16, B 16 x 8.  Lane (g, q) of the warp holds a[2 i], a[2 i + 1]: rows g, g + 8 of column 4 i + q; b[i]: row 4 i + q of
+// column g; c: rows g, g, g + 8, g + 8 of columns 2 q, 2 q + 1.
+__device__ __forceinline__ void mma_f64_16x8x16(double (&c)[4], const double (&a)[8], const double (&b)[4]) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f64.f64.f64.f64 {%0, %1, %2, %3}, {%4, %5, %6, %7, %8, %9, %10, %11}, {%12, %13, %14, %15}, {%0, %1, %2, %3};"
+        : "+d"(c[0]), "+d"(c[1]), "+d"(c[2]), "+d"(c[3])
+        : "d"(a[0]), "d"(a[1]), "d"(a[2]), "d"(a[3]), "d"(a[4]), "d"(a[5]), "d"(a[6]), "d"(a[7]), "d"(b[0]), "d"(b[1]), "d"(b[2]), "d"(b[3]));
+}
 template <bool BF16>
-__device__ __forceinline__ void mma_16x8x16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    if constexpr (BF16)
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
-            : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
-            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
-    else
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
-            : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
-            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+__device__ __forceinline__ void pair_to_double(uint32_t w, double& lo, double& hi) {
+    const float2 f = pair_to_float<BF16>(w);
+    lo = static_cast<double>(f.x);
+    hi = static_cast<double>(f.y);
 }
 
 // Logits of 16 experts (rows a0 and a1 of lane group g: experts g and g + 8) and 8 tokens over pieces [v0, v1) of 8 of K.  Lane (g, q) holds
-// the 8 numbers of piece 4 i + q of its rows and of token g: any order of K serves an MMA if both operands keep it.  An
-// MMA's 16 products are added in fp32, its results in 64 bits: which expert a token gets must not depend on a sum's rounding.
+// the 8 numbers of piece 4 i + q of its rows and of token g: any order of K serves an MMA if both operands keep it.
+// All in 64 bits, where the products are exact: which expert a token gets must not depend on a sum's rounding.
 template <bool BF16, bool VEC>
 __device__ __forceinline__ void moe_logits(const uint16_t* a0, const uint16_t* a1, const uint16_t* x, int k, int v0, int v1, int q, double (&sum)[4]) {
     constexpr int AHEAD = 4;                                      // MMA pairs (32 of K) whose loads are in flight together
@@ -207,13 +210,18 @@ __device__ __forceinline__ void moe_logits(const uint16_t* a0, const uint16_t* a
         }
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
-            float d[4];
-            mma_16x8x16<BF16>(d, a[i].x, c[i].x, a[i].y, c[i].y, b[i].x, b[i].y);
+            const uint32_t wa[4] = {a[i].x, a[i].y, a[i].z, a[i].w}, wc[4] = {c[i].x, c[i].y, c[i].z, c[i].w}, wb[4] = {b[i].x, b[i].y, b[i].z, b[i].w};
 #pragma unroll
-            for (int j = 0; j < 4; ++j) sum[j] += static_cast<double>(d[j]);
-            mma_16x8x16<BF16>(d, a[i].z, c[i].z, a[i].w, c[i].w, b[i].z, b[i].w);
+            for (int half = 0; half < 2; ++half) {
+                double da[8], db[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) sum[j] += static_cast<double>(d[j]);
+                for (int j = 0; j < 2; ++j) {
+                    pair_to_double<BF16>(wa[half * 2 + j], da[4 * j], da[4 * j + 2]);
+                    pair_to_double<BF16>(wc[half * 2 + j], da[4 * j + 1], da[4 * j + 3]);
+                    pair_to_double<BF16>(wb[half * 2 + j], db[2 * j], db[2 * j + 1]);
+                }
+                mma_f64_16x8x16(sum, da, db);
+            }
         }
     }
 }

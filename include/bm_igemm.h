@@ -295,7 +295,7 @@ int bm_f4_gemm(const uint8_t *A, const uint8_t *SA, const float *ra, const uint8
  * X[T x H] and router[E x H] in `x_type` (BM_F16 or BM_BF16), Y[T x H] in the same type, `ldx` / `ldy` elements between
  * rows.  W13: E matrices of 2 I rows (I gate rows, then I up rows) and K = H; W2: E matrices of H rows and K = I;
  * both in `format`, one after the other, scales in BM_SCALE_ROWS; r13 [E * 2 I] and r2 [E * H]: row factors, NULL for ones.
- * ids and weights [T x top]: the selection, in descending order, may be NULL.  Sums in fp32 (logits in 64 bits).  X and the hidden
+ * ids and weights [T x top]: the selection, in descending order, may be NULL.  Sums in fp32 (logits: products and sums in 64 bits).  X and the hidden
  * activations silu(gate) * up enter the products as fixed-point numbers of 24 bits under the largest of their block of 32 (16)
  * neighbours: off by at most 2^-22.7 of it (BM_F4_E4M3: or 2^-39 of their row's largest, if that is more), exact where they are
  * fp16 numbers down to 2^-10 of it or bf16 numbers down to 2^-13; with BM_F4_E8M0 a number above 1.7 * 2^127 (2.9e38) counts as an

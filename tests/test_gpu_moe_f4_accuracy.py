@@ -111,3 +111,55 @@ def test_many_short_runs_beside_a_busy_stream(T, H, I, E, top, fmt):
         again = layer.run(x)
         assert all(torch.equal(a, b) for a, b in zip(first, again))
     assert_clean_status()
+
+
+def test_large_channels_that_cancel_in_the_logits():
+    """Products of 3e6 and -3e6 beside ones around 1: fp32 holds no more than quarters there, and the experts lie closer."""
+    T, H, E, top = 10, 256, 32, 6
+    g = torch.Generator().manual_seed(41)
+    x, router = torch.randn(T, H, generator=g), torch.randn(E, H, generator=g) / 16
+    x[:, 0], x[:, 1], x[:, 77], x[:, 79] = 30000.0, -30000.0, -20000.0, 20000.0
+    router[:, 0] = router[:, 1] = torch.randint(50, 200, (E,), generator=g).float()
+    router[:, 77] = router[:, 79] = torch.randint(50, 200, (E,), generator=g).float()
+    for norm in (True, False):
+        layer = FineLayer(T, H, 48, E, top, torch.float16, ig.BM_F4_E8M0, norm, seed=42, x=x, router=router)
+        y, ids, weights = layer.run()
+        assert_clean_status()
+        logits, order, p = layer.select()
+        assert np.array_equal(ids.cpu().numpy(), order)
+        assert np.allclose(weights.double().cpu().numpy(), p, rtol=2e-6 * (1 + np.abs(logits).max(1)[:, None]), atol=1e-30)
+        assert not y.isnan().any()                                # (most are 10^7 and more, infinities in fp16)
+
+
+def test_equal_logits_from_rows_that_are_not_equal():
+    """Rows with the same numbers in other orders, all of x one: exact in 64 bits (fp16 numbers are multiples of 2^-24), so equal, lowest index first."""
+    T, H, E, top = 3, 1024, 20, 9
+    g = torch.Generator().manual_seed(43)
+    numbers = (torch.randn(H, generator=g) * torch.exp2(torch.rand(H, generator=g) * 24 - 14)).half()
+    router = torch.stack([numbers[torch.randperm(H, generator=g)] for _ in range(E)])
+    router[4, 0] = router[11, 0] = 30000.0
+    layer = FineLayer(T, H, 32, E, top, torch.float16, ig.BM_F4_E4M3, seed=44, x=torch.ones(T, H), router=router)
+    _, ids, weights = layer.run()
+    assert_clean_status()
+    order = sorted(range(E), key=lambda e: (-router[e].double().sum().item(), e))
+    assert ids.tolist() == [order[:top]] * T and sorted(order[:2]) == [4, 11]
+    equal = [n for n, e in enumerate(order[:top]) if e not in (4, 11)]
+    assert (weights[:, equal] == weights[:, equal[:1]]).all()
+
+
+@pytest.mark.parametrize("norm", [True, False])
+def test_bf16_logits_beyond_the_range_of_fp32(norm):
+    """Logits of 2^140 are numbers in 64 bits: the largest takes the whole weight, as with a router 2^-60 times as large."""
+    T, H, I, E, top = 5, 200, 48, 12, 4
+    g = torch.Generator().manual_seed(45)
+    x, router = torch.randn(T, H, generator=g) * 2.0 ** 80, torch.randn(E, H, generator=g) * 2.0 ** 60
+    layer = FineLayer(T, H, I, E, top, torch.bfloat16, ig.BM_F4_E8M0, norm, seed=46, x=x, router=router)
+    layer.reweigh("w13", by_row=torch.full((E * 2 * I,), 2.0 ** -80))
+    y, ids, weights = layer.run()
+    assert_clean_status()
+    assert np.array_equal(ids.cpu().numpy(), layer.select()[1])
+    assert (weights[:, 0] == 1).all() and (weights[:, 1:] == 0).all()
+    layer.router_here = (layer.router.float() * 2.0 ** -60).bfloat16().to(dev())
+    again = layer.run()
+    assert torch.equal(ids, again[1]) and torch.equal(weights, again[2]) and torch.equal(y, again[0])
+    assert y.isfinite().all() and y.abs().max() > 0.01
