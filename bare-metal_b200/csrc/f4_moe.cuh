@@ -770,7 +770,10 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_con
                     }
                     const int k0 = ((at % items[1]) * 32 + lane) * 8;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) h[i] = k0 + i < k ? __fdividef(g[i], 1.f + __expf(-g[i])) * up[i] : 0.f;      // (nobody wrote what is behind)
+                    for (int i = 0; i < 8; ++i) {
+                        const float e = __expf(-fabsf(g[i]));       // not exp(-g): beyond 2^126 the quotient would be zero
+                        h[i] = k0 + i < k ? __fdividef(g[i] < 0.f ? g[i] * e : g[i], 1.f + e) * up[i] : 0.f;      // (nobody wrote what is behind)
+                    }
                 };
                 if constexpr (FMT == FMT_E4M3) {                  // the rows' factors first; the numbers wait in the tile
 #pragma unroll 1

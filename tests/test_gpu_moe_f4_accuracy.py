@@ -163,3 +163,27 @@ def test_bf16_logits_beyond_the_range_of_fp32(norm):
     again = layer.run()
     assert torch.equal(ids, again[1]) and torch.equal(weights, again[2]) and torch.equal(y, again[0])
     assert y.isfinite().all() and y.abs().max() > 0.01
+
+
+@pytest.mark.parametrize("fmt,in_x", [("e8m0", True), ("e8m0", False), ("e4m3", False)])
+def test_gates_far_below_zero(fmt, in_x):
+    """silu(-88) is -88 * 6e-39, and 2^119 times that is a number: SiLU by exp(-g) and one division gives nothing beyond 2^126.  (Not E4M3 with
+    2^100 in x: a number of 88 is then below 2^-39 of its row's largest, and the gates may be anything up to 2^61.)"""
+    gates = [-80.0, -87.0, -87.5, -88.0, -88.5, -12.0, 3.0]
+    T, H, I = len(gates), 64, 32
+    layer = FineLayer(T, H, I, 1, 1, torch.bfloat16, FMT[fmt], seed=51, x=torch.zeros(T, H), router=torch.zeros(1, H))
+    layer.x[:, 0], layer.x[:, 40] = torch.tensor(gates).bfloat16(), 2.0 ** 100 if in_x else 1.0
+    w13, w2 = torch.zeros(2 * I, H), torch.zeros(H, I)
+    w13[:I, 0], w13[I:, 40], w2[:, 5] = 1.0, 2.0 ** 19 if in_x else 2.0 ** 119, 1.0
+    for name, w in (("w13", w13), ("w2", w2)):
+        layer.plain[name] = w.bfloat16()
+        layer.w[name] = ig.quantize_f4(layer.plain[name].to(dev()), layer.fmt, ig.BM_SCALE_ROWS)
+    y, _, _ = layer.run()
+    assert_clean_status()
+    # the exponential 8 + |g| units; the weights 1 and 2^119 are off by up to a sixteenth in E4M3 (as read back); the output's rounding
+    one, much = (ig.dequantize_f4(*layer.w["w13"], 2 * I, H, torch.float32, layer.fmt, ig.BM_SCALE_ROWS)[r, k].item() for r, k in ((0, 0), (I, 40)))
+    last = ig.dequantize_f4(*layer.w["w2"], H, I, torch.float32, layer.fmt, ig.BM_SCALE_ROWS)[0, 5].item()
+    g = np.array(gates) * one
+    want = (g / (1 + np.exp(-g)) * (2.0 ** 100 if in_x else 1.0) * much * last)[:, None]
+    bound = np.abs(want) * ((8 + np.abs(g[:, None])) * 2.0 ** -24 + 2.0 ** -8 * 1.01 + 2.0 ** -22)
+    assert (np.abs(y.double().cpu().numpy() - want) <= bound).all()
