@@ -411,7 +411,14 @@ def f4_linear(Xq, Xs, Xr, Wq, Ws, Wr, D, M, N, K, fmt=BM_F4_E4M3):
 
 @functools.lru_cache(maxsize=1024)
 def _moe_f4_bytes(T, H, inter, E, top):
-    return _lib.load().bm_moe_f4_workspace_bytes(T, H, inter, E, top)
+    """Bytes of the workspace."""
+    need = 0
+    if all(0 < v < 2 ** 31 for v in (T, H, inter, E, top)):      # what the entry points' arguments hold
+        need = _lib.load().bm_moe_f4_workspace_bytes(T, H, inter, E, top)
+    if not need:
+        raise BmError(f"no expert layer has {T} tokens of {H}, {E} experts of {inter} and {top} of them a token: at most 64 tokens, 256 "
+                      "experts, 16 (and no more than there are) a token, sizes from 1 to 16384")
+    return need
 
 
 def moe_f4(X, router, w13, w2, top, inter, fmt=BM_F4_E4M3, normalize=True, out=None, workspace=None):
@@ -426,7 +433,7 @@ def moe_f4(X, router, w13, w2, top, inter, fmt=BM_F4_E4M3, normalize=True, out=N
         raise BmError("X must be float16 or bfloat16")
     ldx = _f4_rows(X, "X")
     T, H = X.shape
-    if router.dim() != 2 or router.shape[1] != H:
+    if _here(router, "router").dim() != 2 or router.shape[1] != H:
         raise BmError(f"router must be a matrix [experts, {H}]")
     E = router.shape[0]
     device = _device()
@@ -437,10 +444,10 @@ def moe_f4(X, router, w13, w2, top, inter, fmt=BM_F4_E4M3, normalize=True, out=N
         out = _new(X, (T, H), X.dtype)
     elif _here(out, "out").dtype != X.dtype or tuple(out.shape) != (T, H):
         raise BmError(f"out must be a {X.dtype} matrix [{T}, {H}]")
-    ids, weights = _new(X, (T, top), torch.int32), _new(X, (T, top), torch.float32)
     need = _moe_f4_bytes(T, H, inter, E, top)
+    ids, weights = _new(X, (T, top), torch.int32), _new(X, (T, top), torch.float32)
     if workspace is None:
-        workspace = _new(X, (max(need, 256),), torch.uint8)
+        workspace = _new(X, (need,), torch.uint8)
     rc = L.bm_moe_f4(X.data_ptr(), router_ptr, _ELEMENT[X.dtype], *a13, *a2, out.data_ptr(), ids.data_ptr(), weights.data_ptr(),
                      T, H, inter, E, top, ldx, _f4_rows(out, "out"), fmt, int(bool(normalize)),
                      _buffer(workspace, torch.uint8, need, "workspace", device), workspace.numel(), _stream())
