@@ -904,7 +904,9 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_con
                         float sum = __uint_as_float(v[kMoeParts - 1]);        // the smallest first
 #pragma unroll
                         for (int i = kMoeParts - 2; i >= 0; --i) sum = fmaf(sum, 0.125f, __uint_as_float(v[i]));
-                        if (in) __stcg(out + slot_row[j] * step, sum * factor * slot_scale[j]);
+                        // factors on different sides of one are multiplied first, others one by one: nothing leaves fp32's range that the result is in
+                        const float scale = slot_scale[j];
+                        if (in) __stcg(out + slot_row[j] * step, (factor < 1.f) != (scale < 1.f) ? sum * (factor * scale) : sum * factor * scale);
                     }
                     tc_fence_before_sync();
                     __syncwarp();

@@ -283,7 +283,8 @@ int bm_dequantize_f4(const uint8_t *Q, const uint8_t *S, const float *row_scale,
                      int64_t ldo, int format, int scale_layout, void *stream);
 
 /* D[m][n] = (sum_k A[m][k] * W[n][k], both times their scales, added in fp32) * (ra[m] * rw[n]), rounded once to
- * `d_type`.  A[M x K] and W[N x K] in `format` with BM_SCALE_TILED scales; ra, rw: row factors, NULL for ones. */
+ * `d_type`.  A[M x K] and W[N x K] in `format` with BM_SCALE_TILED scales; ra, rw: row factors, NULL for ones (their product is
+ * formed first, in fp32). */
 int bm_f4_gemm(const uint8_t *A, const uint8_t *SA, const float *ra, const uint8_t *W, const uint8_t *SW, const float *rw,
                void *D, int d_type, int M, int N, int K, int64_t ldd, int format, void *stream);
 

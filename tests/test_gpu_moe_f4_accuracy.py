@@ -53,11 +53,13 @@ def test_small_activations_beside_much_larger_ones(T, H, I, fmt, dtype):
     layer.check(*out)
 
 
-@pytest.mark.parametrize("scale", [2.0 ** -110, 2.0 ** -122])
-def test_tiny_bf16_activations_under_weights_with_large_scales(scale):
-    """E8M0 blocks whose scale times 2^-22 is no normal fp32 number, brought back into range by the weights' scales and factors."""
-    layer = FineLayer(3, 128, 64, 4, 2, torch.bfloat16, ig.BM_F4_E8M0, seed=21, spread=0.0)
-    layer.router = (layer.router.float() * 2.0 ** 100).bfloat16()
+@pytest.mark.parametrize("fmt", list(FMT))
+@pytest.mark.parametrize("scale", [2.0 ** -110, 2.0 ** -122, 2.0 ** 115])
+def test_tiny_and_huge_bf16_activations_under_weights_that_bring_them_back(scale, fmt):
+    """E8M0 blocks whose scale times 2^-22 is no normal fp32 number; E4M3 rows whose factor, or whose weights' factors, are beyond it with the sums.
+    (Below 2^-119 E4M3's row factor stays at 2^-126, and every bf16 number is a multiple of 2^-133: exact.)"""
+    layer = FineLayer(3, 128, 64, 4, 2, torch.bfloat16, FMT[fmt], seed=21, spread=0.0)
+    layer.router = (layer.router.float() * (2.0 ** 100 if scale < 1 else 2.0 ** -100)).bfloat16()
     layer.router_here = layer.router.to(dev())
     layer.x = (layer.x.float() * scale).bfloat16()
     layer.reweigh("w13", by_row=torch.full((4 * 128,), 1.0 / scale))
