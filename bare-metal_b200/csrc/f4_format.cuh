@@ -65,19 +65,6 @@ __device__ __forceinline__ void e2m1x8_to_half(uint32_t w, uint32_t (&h)[4]) {
         : "r"(w));
 }
 
-// The same by integer arithmetic, 2^-14 times the values, in the order (1, 5) (3, 7) (0, 4) (2, 6): a code's sign and its three
-// other bits are the sign and, with the exponent's low two bits, the top of the mantissa of fp16's high byte (codes below 1
-// land in its subnormal numbers, which have the same spacing).  Also where the codes come straight from e2m1x8: from
-// there the conversion back was compiled to one that takes two of the four bytes for zeros.
-__device__ __forceinline__ void e2m1x8_to_small_half(uint32_t w, uint32_t (&h)[4]) {
-    const uint32_t odd = (w & 0x80808080u) | ((w >> 3) & 0x0E0E0E0Eu);
-    const uint32_t even = ((w << 4) & 0x80808080u) | ((w << 1) & 0x0E0E0E0Eu);
-    h[0] = __byte_perm(odd, 0, 0x2404);
-    h[1] = odd & 0xFF00FF00u;
-    h[2] = __byte_perm(even, 0, 0x2404);
-    h[3] = even & 0xFF00FF00u;
-}
-
 // two 16-bit numbers of one word as fp32
 template <bool BF16>
 __device__ __forceinline__ float2 pair_to_float(uint32_t w) {
