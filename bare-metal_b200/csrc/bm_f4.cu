@@ -181,7 +181,9 @@ static int f4_few(const F4Operands& o, const F4GemmParams& g, DeviceState* dev, 
 
 // Which kernel (1 few tokens, 2 tiles of 128 x 128, 3 CTA pairs).  Microseconds, fitted to 1 to 2048 tokens on weights from 1024 x 1024 to
 // 28672 x 8192 (E4M3, fp16 out): start-up plus waves, each a fixed part (the drain) and 256-wide blocks of K; half a wave where the pair
-// kernel cuts its last one.
+// kernel cuts its last one.  Used for E8M0 and fp32 results too: over 192 combinations of both formats and outputs on six weights and 1 to 2048
+// tokens the choice was within 7 % of the best kernel but twice, 5.3 against 4.7 us (48 x 2260 x 1000, E8M0) and 33.0 against 30.2
+// (128 x 28672 x 8192), though the model itself can be off by more (777 x 2260 x 1000 into fp32: 4.1 us, measured 5.3).
 static int f4_choose(int M, int N, int K, int sms) {
     const float kb = static_cast<float>(ceil_div(K, kF4BK));
     const long long lone_tiles = static_cast<long long>(ceil_div(M, 128)) * ceil_div(N, 128);

@@ -16,8 +16,9 @@
 // Where at most half of the pairs would work in the last wave, its tiles are cut into two halves of 128 columns for two pairs.
 //
 // What bounds it: an SM needs 128 x 256 x 64 MACs = 128 clocks an MMA (512 a stage) and 38 KiB of operands a stage, 76 B/clk.
-// Measured (product alone): 4096^3 28.3 us (without its loads 28, without the epilogue 26), 8192 x 22016 x 4096 275 us, 8192^3 209 us,
-// 5.3 PFLOP/s (power-capped when sustained); 777 x 2260 x 1000 6.5 us.
+// Measured (product alone, fp16 out; in brackets without its loads, and without the epilogue): 4096^3 28.4 us (24.0, 25.4), 8192 x 22016 x 4096
+// E8M0 276 us (195, 238), 8192^3 201 to 209 us (150, 179), 5.3 to 5.5 PFLOP/s (power-capped when sustained); 777 x 2260 x 1000
+// 6.6 us (5.5, 4.3).
 #pragma once
 #include "epilogue.cuh"
 #include "f4_format.cuh"

@@ -30,13 +30,13 @@
 // tensor memory by four warps (tcgen05.st) on the way.  The ring runs ahead into the next expert and, over the wait
 // for the other CTAs' gate / up sums, into the down projection's weights.
 //   The gate / up sums go to the workspace in fp32; whoever needs an expert's hidden activations waits for its sums, applies
-// SiLU and cuts them into digits.  The experts' outputs go to the workspace in fp32 and are added per token, in the order of the
-// selection, after a last wait: no atomics on sums, the same bits on every call.
-//   Measured (device, both kernels): 64 tokens on 64 experts of 4096 x 1408, top 6, E8M0, 589 MB: 130 us, 4.5 TB/s; 16 tokens on 128 experts
-// of 2048 x 768, top 8, E4M3, 221 MB: 60 us, 3.7 TB/s; 1 token, 59 MB: 32 us.  About 15 us of each is not streaming: the router kernel and
-// the hand-over 6, the wait between the phases for the last sums and the first activations 4, the last wait and the sum over the
-// experts 5.  Beyond that it is the chain of a stage (TMA, scales to tensor memory, MMA, release), not the bytes: with the
-// loads taken out 64 tokens still took 102 us and 16 tokens 55.
+// SiLU and cuts them into digits.  The experts' outputs go to the workspace in fp32 and are added per token after a last wait, every fourth
+// choice by one lane and the four sums in a fixed tree: no atomics on sums, the same bits on every call.
+//   Measured (device, both kernels): 64 tokens on 64 experts of 4096 x 1408, top 6, E8M0, 589 MB: 133 us, 4.4 TB/s; 16 tokens on 128 experts
+// of 2048 x 768, top 8, E4M3, 221 MB: 62.6 us, 3.5 TB/s; 1 token, 59 MB: 34.2 us.  About 17 us of each is not streaming: the router kernel and
+// the hand-over 8, the wait between the phases for the last sums and the first activations 4, the last wait and the sum over the
+// experts 5.  Beyond that it is the chain of a stage (TMA, scales to tensor memory, MMA, release) more than the bytes: with the
+// loads taken out 64 tokens take 98 us, 16 tokens 51 and 1 token 29.
 #pragma once
 #include "f4_format.cuh"
 #include "f4_gemm.cuh"
